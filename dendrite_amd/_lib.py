@@ -77,6 +77,12 @@ class dh_plan_item(C.Structure):
                                           "kv_head", "flags", "tail_seq")]
 
 
+class dh_token_tables(C.Structure):
+    _fields_ = [("indices", C.c_void_p), ("indptr", C.c_void_p), ("kv_len", C.c_void_p), ("q_indptr", C.c_void_p),
+                ("batch_size", C.c_uint32), ("num_indices", C.c_uint32), ("rows", C.c_uint32),
+                ("max_kv_len", C.c_uint32)]
+
+
 class dh_node_info(C.Structure):
     _fields_ = [("id", C.c_uint64), ("parent", C.c_uint64), ("num_tokens", C.c_uint64),
                 ("num_children", C.c_uint32), ("is_active", C.c_uint32)]
@@ -130,6 +136,11 @@ SIGNATURES = {
     "dh_csr_workspace_size": (C.c_size_t, [C.POINTER(dh_attn_config), _U32, _U32]),
     "dh_decode_csr": (_I, [_P, _P, C.POINTER(dh_attn_config), _U32, _P, _P, _P, _P, _P, _P, C.c_size_t, _P,
                            _P]),
+    "dh_pool_append_tokens": (_I, [_P, C.POINTER(dh_token_tables), _P, _P, _U64, _U64, _U32, _P, _P]),
+    "dh_pool_read_tokens": (_I, [_P, C.POINTER(dh_token_tables), _P, _P, _U64, _U64, _U32, _P, _P]),
+    "dh_window_workspace_size": (C.c_size_t, [C.POINTER(dh_attn_config), C.POINTER(dh_token_tables), _U32]),
+    "dh_attend_window": (_I, [_P, _P, C.POINTER(dh_attn_config), _U32, C.POINTER(dh_token_tables), _P, _U64, _P, _U64,
+                              _P, C.c_size_t, _P, _P]),
     "dh_merge_states": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _P]),
     "dh_gather_debug": (_I, [_P, _PU32, _U32, _U32, _P, _PU32, _P]),
     "dh_debug_e4m3_to_bf16": (_I, [_I, _P, _P, _U32, _P]),

@@ -75,6 +75,83 @@ def _stream_ptr(stream) -> Optional[int]:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+def _device_stream(stream, device: int) -> Optional[int]:
+    """The hipStream_t of `stream`; None: torch's current stream on `device`,
+    whichever device is current."""
+    if stream is None:
+        return _torch().cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _on_device(t, device: int, what: str) -> None:
+    if not t.is_cuda or t.device.index != device:
+        raise DhError(_lib.DH_EINVAL, f"{what} is on {t.device}, not on cuda:{device}")
+
+
+def _rows(t, heads: int, dim: int, device: int, what: str) -> int:
+    """Checks rows [n, heads, dim] whose elements lie together in each row;
+    returns the row stride in elements."""
+    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, dim):
+        raise DhError(_lib.DH_EINVAL, f"{what} shape {tuple(t.shape)} is not [rows, {heads}, {dim}]")
+    _on_device(t, device, what)
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        raise DhError(_lib.DH_EINVAL, f"{what}: the elements of a row must be contiguous (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+class TokenTables:
+    """dh_token_tables: where sequences' tokens are and which of them are new,
+    in device int32 tensors that every call reads anew.
+
+    indices [n] and indptr [B + 1]: token t of sequence b is slot t % 16 of
+    page indices[indptr[b] + t // 16].  kv_len [B]: its tokens, the new ones
+    included.  q_indptr [B + 1]: its last q_indptr[b + 1] - q_indptr[b] tokens
+    are the call's rows q_indptr[b].. (None: one new token a sequence, row b;
+    kv_len[b] = 0 marks an unused row).  max_kv_len: no sequence holds more
+    tokens (default: what MAX_SEQ_LEN allows); it sizes the work of
+    attend_window, so a bound near the truth is faster."""
+
+    def __init__(self, indices, indptr, kv_len, q_indptr=None, max_kv_len: int = _lib.MAX_SEQ_LEN):
+        torch = _torch()
+        named = {"indices": indices, "indptr": indptr, "kv_len": kv_len, "q_indptr": q_indptr}
+        for name, t in named.items():
+            if t is None and name == "q_indptr":
+                continue
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
+                raise DhError(_lib.DH_EINVAL, f"{name} must be a contiguous int32 device vector")
+            if t.device != indptr.device:
+                raise DhError(_lib.DH_EINVAL, f"{name} is on {t.device}, indptr on {indptr.device}")
+        self.batch_size = kv_len.numel()
+        for name, t in (("indptr", indptr), ("q_indptr", q_indptr)):
+            if t is not None and t.numel() != self.batch_size + 1:
+                raise DhError(_lib.DH_EINVAL, f"{name} has {t.numel()} entries for {self.batch_size} sequences")
+        if not 0 <= int(max_kv_len) < 1 << 31:
+            raise DhError(_lib.DH_EINVAL, f"max_kv_len {max_kv_len} is outside 0 .. 2^31 - 1")
+        self.indices, self.indptr, self.kv_len, self.q_indptr = indices, indptr, kv_len, q_indptr
+        self.max_kv_len = int(max_kv_len)
+        self.device = indptr.device.index
+        c = _lib.dh_token_tables()
+        c.indices, c.indptr, c.kv_len = indices.data_ptr() or None, indptr.data_ptr(), kv_len.data_ptr() or None
+        c.q_indptr = None if q_indptr is None else q_indptr.data_ptr()
+        c.batch_size, c.num_indices, c.max_kv_len = self.batch_size, indices.numel(), self.max_kv_len
+        self._c = c
+
+    def to_c(self, rows: int) -> _lib.dh_token_tables:
+        c = _lib.dh_token_tables()
+        C.pointer(c)[0] = self._c
+        c.rows = rows
+        return c
+
+
+def _status_ptr(status, device: int):
+    if status is None:
+        return None
+    if status.dtype != _torch().int32 or status.numel() < 1:
+        raise DhError(_lib.DH_EINVAL, "status must be an int32 tensor")
+    _on_device(status, device, "status")
+    return status.data_ptr()
+
+
 class AttentionConfig:
     """AttentionConfig (backend.rs:17-59) plus the GQA mapping and dtypes."""
 
@@ -221,6 +298,35 @@ class Pool:
                                          _stream_ptr(stream) if stream is not None else None))
         if stream is None:
             self.backend.synchronize()
+
+    def _token_rows(self, call, tables: "TokenTables", k, v, status, stream) -> None:
+        dev = self.backend.device
+        if tables.device != dev:
+            raise DhError(_lib.DH_EINVAL, f"tables are on cuda:{tables.device}, the pool on cuda:{dev}")
+        if k.dtype != v.dtype or k.shape != v.shape:
+            raise DhError(_lib.DH_EINVAL, f"k is {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
+        ks = _rows(k, self.num_kv_heads, self.head_dim, dev, "k")
+        vs = _rows(v, self.num_kv_heads, self.head_dim, dev, "v")
+        try:
+            code = dtype_code(k.dtype)
+        except KeyError:
+            raise DhError(_lib.DH_EINVAL, f"row dtype {k.dtype} (float32, bfloat16 or float16)") from None
+        check(call(self._h, C.byref(tables.to_c(k.shape[0])), k.data_ptr(), v.data_ptr(), ks, vs, code,
+                   _status_ptr(status, dev), _device_stream(stream, dev)))
+
+    def append_tokens(self, tables: "TokenTables", k, v, status=None, stream=None) -> None:
+        """Writes the new tokens' K and V (rows [rows, num_kv_heads, head_dim]
+        float32 / bfloat16 / float16, views of wider rows allowed) into their
+        pages in the pool's format (dh_pool_append_tokens).  A page written
+        must belong to one sequence.  status: device int32 that receives
+        DH_EINVAL where the tables refuse a sequence or name a page outside
+        the pool, and is left alone otherwise."""
+        self._token_rows(lib().dh_pool_append_tokens, tables, k, v, status, stream)
+
+    def read_tokens(self, tables: "TokenTables", k, v, status=None, stream=None) -> None:
+        """Reads the tables' tokens back into rows k and v, dequantised in f32
+        and rounded to their dtype (dh_pool_read_tokens)."""
+        self._token_rows(lib().dh_pool_read_tokens, tables, k, v, status, stream)
 
     def copy_page(self, src: int, dst: int, stream=None) -> None:
         check(lib().dh_pool_copy_page(self._h, src, dst,
@@ -426,6 +532,39 @@ def decode_csr(backend: "Backend", pool: "Pool", config: AttentionConfig, q, ind
                               ptr(indptr), ptr(last_page_len), ptr(out), ptr(workspace),
                               workspace.numel() * workspace.element_size(), ptr(status),
                               C.c_void_p(_stream_ptr(stream))))
+
+
+def window_workspace_size(config: AttentionConfig, tables: TokenTables, rows: int, sinks: int = 0) -> int:
+    """dh_window_workspace_size: workspace bytes of attend_window."""
+    return int(lib().dh_window_workspace_size(C.byref(config.to_c()), C.byref(tables.to_c(rows)), sinks))
+
+
+def attend_window(backend: Backend, pool: Pool, config: AttentionConfig, tables: TokenTables, q, out, workspace=None,
+                  sinks: int = 0, status=None, stream=None) -> None:
+    """Causal attention of the tables' new tokens over their sequences' pages
+    under config.sliding_window (None: all earlier tokens), with each
+    sequence's first `sinks` tokens always in sight (dh_attend_window).  q /
+    out: rows [rows, num_heads, head_dim] of config.q_dtype (views of wider
+    rows allowed), the new tokens' K / V already in the pages
+    (Pool.append_tokens).  workspace: device uint8 of >= window_workspace_size
+    bytes; calls that may overlap need one each.  status: as append_tokens."""
+    dev = backend.device
+    if tables.device != dev:
+        raise DhError(_lib.DH_EINVAL, f"tables are on cuda:{tables.device}, the backend on cuda:{dev}")
+    if q.dtype != torch_dtype(config.q_dtype) or out.dtype != q.dtype or q.shape != out.shape:
+        raise DhError(_lib.DH_EINVAL, f"q is {q.dtype} {tuple(q.shape)}, out {out.dtype} {tuple(out.shape)}, the "
+                      f"config's {torch_dtype(config.q_dtype)}")
+    if sinks < 0:
+        raise DhError(_lib.DH_EINVAL, f"sinks {sinks} is negative")
+    qs = _rows(q, config.num_heads, config.head_dim, dev, "q")
+    os_ = _rows(out, config.num_heads, config.head_dim, dev, "out")
+    ws, nbytes = None, 0
+    if workspace is not None:
+        _on_device(workspace, dev, "workspace")
+        ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(lib().dh_attend_window(backend._h, pool._h, C.byref(config.to_c()), min(sinks, 0xFFFFFFFF),
+                                 C.byref(tables.to_c(q.shape[0])), q.data_ptr(), qs, out.data_ptr(), os_, ws, nbytes,
+                                 _status_ptr(status, dev), _device_stream(stream, dev)))
 
 
 class TreeDecoder:
@@ -990,5 +1129,5 @@ class HipBackend:
         return out.reshape(bsz, S, hq, d).permute(0, 2, 1, 3).contiguous()
 
 
-__all__ = ["AttentionConfig", "Backend", "Pool", "DecodePlan", "PrefillPlan", "decode_batch", "HipBackend",
+__all__ = ["AttentionConfig", "Backend", "Pool", "TokenTables", "attend_window", "window_workspace_size", "DecodePlan", "PrefillPlan", "decode_batch", "HipBackend",
            "is_available", "dtype_code", "torch_dtype", "raw_to_tensor"]

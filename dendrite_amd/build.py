@@ -38,6 +38,8 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", f"-I{os.path.join(ROOT, 'includ
 # operand canonicalisation.
 DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           "-fno-honor-nans", "-mno-amdgpu-ieee"]
+# token_kernels.hip is built without that: what it does with NaN is stated.
+EXACT = {"token_kernels.hip": [f for f in DEVICE if f not in ("-fno-honor-nans", "-mno-amdgpu-ieee")]}
 HOST = ["-D__HIP_PLATFORM_AMD__", f"-I{os.path.join(ROCM, 'include')}", "-x", "c++"]
 
 # Host-only instrumentation: every -fsanitize= on a hipcc line sits behind
@@ -47,7 +49,8 @@ SANITIZE = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=unde
 SAN_BUILD = os.path.join(PKG, "_build_san")
 SAN_LIB = os.path.join(SAN_BUILD, "libdendrite_hip.so")
 
-HIP_SOURCES = ["decode_kernels.hip", "csr_kernels.hip", "write_kernels.hip"]
+HIP_SOURCES = ["decode_kernels.hip", "csr_kernels.hip", "write_kernels.hip", "token_kernels.hip",
+               "window_narrow.hip", "window_wide.hip"]
 HOST_SOURCES = ["api.cpp", "planner.cpp", "block_model.cpp"]
 TESTDATA_SOURCES = ["synth.cpp"]
 
@@ -72,7 +75,7 @@ def build(verbose: bool = False, sanitize: bool = False) -> str:
     jobs = []
     for src in HIP_SOURCES:
         obj = os.path.join(bdir, src + ".o")
-        jobs.append(([HIPCC, *COMMON, *DEVICE, "-c", os.path.join(CSRC, src), "-o", obj], obj))
+        jobs.append(([HIPCC, *COMMON, *EXACT.get(src, DEVICE), "-c", os.path.join(CSRC, src), "-o", obj], obj))
     for src in HOST_SOURCES:
         obj = os.path.join(bdir, src + ".o")
         jobs.append(([HIPCC, *COMMON, *host_flags, "-c", os.path.join(CSRC, src), "-o", obj], obj))

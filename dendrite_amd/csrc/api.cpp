@@ -1254,6 +1254,204 @@ dh_status dh_decode_csr(dh_backend* be, const dh_pool* pool, const dh_attn_confi
     return DH_OK;
 }
 
+/* ------------------------------------------- token operators, device tables */
+
+namespace {
+
+// What one of the calls needs of its tables on the host.  nullptr arrays are
+// allowed where there is nothing in them.
+dh_status check_tables(const dh_token_tables* t) {
+    if (!t) return fail(DH_EINVAL, "tables is NULL");
+    if (t->batch_size > 0x00FFFFFFu) return fail(DH_EINVAL, "batch_size %u exceeds %u", t->batch_size, 0x00FFFFFFu);
+    if (t->num_indices > 0x7FFFFFFFu || t->rows > 0x7FFFFFFFu || t->max_kv_len > 0x7FFFFFFFu)
+        return fail(DH_EINVAL, "num_indices, rows and max_kv_len must be below 2^31");
+    if (t->batch_size == 0 || t->rows == 0) return DH_OK;
+    if (!t->indptr || !t->kv_len || (t->num_indices && !t->indices))
+        return fail(DH_EINVAL, "indices, indptr and kv_len must be device pointers");
+    if ((reinterpret_cast<uintptr_t>(t->indices) | reinterpret_cast<uintptr_t>(t->indptr) |
+         reinterpret_cast<uintptr_t>(t->kv_len) | reinterpret_cast<uintptr_t>(t->q_indptr)) & 3)
+        return fail(DH_EINVAL, "indices, indptr, kv_len and q_indptr must be 4-byte aligned");
+    if (!t->q_indptr && t->rows < t->batch_size)
+        return fail(DH_EINVAL, "%u rows for one new token of each of %u sequences", t->rows, t->batch_size);
+    return DH_OK;
+}
+
+// Device pointers of the tables and the status word (the pool's device current).
+dh_status check_table_ptrs(const dh_token_tables* t, const int32_t* status) {
+    if (reinterpret_cast<uintptr_t>(status) & 3) return fail(DH_EINVAL, "status must be 4-byte aligned");
+    for (const auto& [ptr, what] : {std::pair<const void*, const char*>{t->num_indices ? t->indices : nullptr, "indices"},
+                                    {t->indptr, "indptr"}, {t->kv_len, "kv_len"}, {t->q_indptr, "q_indptr"},
+                                    {status, "status"}}) {
+        if (!ptr) continue;
+        const dh_status st = check_device_ptr(ptr, what);
+        if (st != DH_OK) return st;
+    }
+    return DH_OK;
+}
+
+// Rows of `width` elements, `stride` elements apart, of a buffer `what`.
+dh_status check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dtype, const char* what) {
+    const uint64_t eb = dh::dtype_bytes(dtype);
+    if (!p) return fail(DH_EINVAL, "%s must be a device pointer", what);
+    if (stride < width) return fail(DH_EINVAL, "%s: row stride %llu is less than a row of %llu elements", what,
+                                    (unsigned long long)stride, (unsigned long long)width);
+    if (stride > (uint64_t(1) << 40)) return fail(DH_EINVAL, "%s: row stride %llu is too large", what,
+                                                  (unsigned long long)stride);
+    if ((reinterpret_cast<uintptr_t>(p) & 15) || (stride * eb & 15))
+        return fail(DH_EINVAL, "%s: rows and their stride must be multiples of 16 bytes", what);
+    return check_device_ptr(p, what);
+}
+
+dh::TokenTables device_tables(const dh_token_tables* t) {
+    return dh::TokenTables{t->indices, t->indptr, t->kv_len, t->q_indptr, t->batch_size, t->num_indices, t->rows,
+                           t->max_kv_len};
+}
+
+dh_status token_copy(const dh_pool* p, const dh_token_tables* t, const void* k, const void* v, uint64_t k_stride,
+                     uint64_t v_stride, uint32_t dtype, int32_t* status, void* stream, bool append) {
+    if (!p) return fail(DH_EINVAL, "pool is NULL");
+    dh_status st = check_tables(t);
+    if (st != DH_OK) return st;
+    if (dtype > DH_DTYPE_F32) return fail(DH_EINVAL, "bad row dtype %u", dtype);
+    if (t->batch_size == 0 || t->rows == 0) return DH_OK;
+    DH_DEVICE(p->be->device);
+    const uint64_t width = uint64_t(p->hkv) * p->d;
+    st = check_rows(k, k_stride, width, dtype, "k");
+    if (st == DH_OK) st = check_rows(v, v_stride, width, dtype, "v");
+    if (st == DH_OK) st = check_table_ptrs(t, status);
+    if (st != DH_OK) return st;
+    const uint64_t eb = dh::dtype_bytes(dtype);
+    dh::TokenCopyArgs a{};
+    a.t = device_tables(t);
+    a.k = static_cast<uint8_t*>(const_cast<void*>(k));
+    a.v = static_cast<uint8_t*>(const_cast<void*>(v));
+    a.k_stride = k_stride * eb;
+    a.v_stride = v_stride * eb;
+    a.data = p->data;
+    a.scales = p->scales;
+    a.num_pages = p->num_pages;
+    a.hkv = p->hkv;
+    a.status = status;
+    const hipError_t e = hipError_t(append ? dh::launch_append_tokens(a, dtype, p->fmt, p->d, stream)
+                                           : dh::launch_read_tokens(a, dtype, p->fmt, p->d, stream));
+    if (e != hipSuccess) return fail(DH_EHIP, "token %s launch failed: %s", append ? "write" : "read", hipGetErrorString(e));
+    return DH_OK;
+}
+
+// How dh_attend_window runs a call: from counts the host has, so the
+// workspace is sized by the same rule.
+struct WindowPlan {
+    bool wide;
+    uint32_t splits;
+    uint32_t window, sinks;
+    size_t o_bytes, bytes;     // workspace: O, all
+};
+
+WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32_t sinks) {
+    WindowPlan w{};
+    const uint64_t r = c.num_heads / c.num_kv_heads, rows = uint64_t(t.rows) * r;
+    // A window that holds the longest sequence is none.
+    w.window = c.sliding_window >= t.max_kv_len ? 0u : c.sliding_window;
+    w.sinks = w.window ? std::min(sinks, t.max_kv_len) : 0u;
+    // Wide blocks (256 or 128 rows) where the sequences fill a good part of
+    // one, narrow ones (16 rows, each reading the cache by itself) below.
+    w.wide = t.q_indptr && c.q_dtype != DH_DTYPE_F32 && rows >= 64 * uint64_t(t.batch_size);
+    const uint64_t block = w.wide ? dh::wide_rows(c.head_dim) : dh::kNarrowRows;
+    const uint64_t all = (uint64_t(t.max_kv_len) + 15) / 16;
+    const uint64_t tokens = (block + r - 2) / r + 1;      // most positions a block covers
+    const uint64_t pages = w.window ? std::min(all, (w.sinks + 15) / 16 + (w.window + tokens + 14) / 16 + 1) : all;
+    const uint64_t blocks = (t.q_indptr ? rows / block + t.batch_size : t.batch_size * ((r + block - 1) / block)) *
+                            c.num_kv_heads;
+    const uint64_t cap = w.wide ? dh::kWideMaxPages - 8 : dh::kWaves * (dh::kNarrowWavePages - 2);
+    const uint64_t least = std::max<uint64_t>(1, (pages + cap - 1) / cap);
+    const uint64_t want = (w.wide ? 256u : 512u) / std::max<uint64_t>(1, blocks);
+    const uint64_t most = pages / (w.wide ? 32 : 16);     // a part worth its own state
+    w.splits = uint32_t(std::max(least, std::min(want, most)));
+    if (w.splits > 1) {
+        const size_t states = size_t(t.rows) * c.num_heads * w.splits;
+        w.o_bytes = align256(states * c.head_dim * sizeof(float));
+        w.bytes = w.o_bytes + align256(states * 2 * sizeof(float));
+    }
+    return w;
+}
+
+}  // namespace
+
+dh_status dh_pool_append_tokens(dh_pool* p, const dh_token_tables* t, const void* k, const void* v, uint64_t k_stride,
+                                uint64_t v_stride, uint32_t src_dtype, int32_t* status, void* stream) {
+    return token_copy(p, t, k, v, k_stride, v_stride, src_dtype, status, stream, true);
+}
+
+dh_status dh_pool_read_tokens(const dh_pool* p, const dh_token_tables* t, void* k, void* v, uint64_t k_stride,
+                              uint64_t v_stride, uint32_t dst_dtype, int32_t* status, void* stream) {
+    return token_copy(p, t, k, v, k_stride, v_stride, dst_dtype, status, stream, false);
+}
+
+size_t dh_window_workspace_size(const dh_attn_config* cfg, const dh_token_tables* t, uint32_t sinks) {
+    if (!cfg || !t || cfg->num_kv_heads == 0 || cfg->num_heads == 0 || t->batch_size == 0 || t->rows == 0) return 0;
+    return plan_window(*cfg, *t, sinks).bytes;
+}
+
+dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_config* cfg, uint32_t sinks,
+                           const dh_token_tables* t, const void* q, uint64_t q_stride, void* out, uint64_t out_stride,
+                           void* ws, size_t ws_bytes, int32_t* status, void* stream) {
+    if (!be || !pool || !cfg) return fail(DH_EINVAL, "NULL argument");
+    if (pool->be != be) return fail(DH_EINVAL, "pool belongs to another backend");
+    dh_status st = validate_config(cfg);
+    if (st != DH_OK) return st;
+    st = check_pool_matches(cfg, pool);
+    if (st != DH_OK) return st;
+    st = check_tables(t);
+    if (st != DH_OK) return st;
+    if (t->batch_size == 0 || t->rows == 0) return DH_OK;
+    const dh_attn_config& c = *cfg;
+    const uint32_t r = c.num_heads / c.num_kv_heads;
+    if (uint64_t(t->rows) * r > 0x7FFFFFFFull) return fail(DH_EUNSUPPORTED, "%u rows of %u heads a KV head", t->rows, r);
+    const WindowPlan w = plan_window(c, *t, sinks);
+    if (ws_bytes < w.bytes || (w.bytes && !ws))
+        return fail(DH_EINVAL, "workspace of %zu bytes is smaller than the %zu bytes the call needs "
+                    "(dh_window_workspace_size)", ws_bytes, w.bytes);
+    if (w.bytes && (reinterpret_cast<uintptr_t>(ws) & 255)) return fail(DH_EINVAL, "workspace must be 256-byte aligned");
+    DH_DEVICE(be->device);
+    const uint64_t width = uint64_t(c.num_heads) * c.head_dim;
+    st = check_rows(q, q_stride, width, c.q_dtype, "q");
+    if (st == DH_OK) st = check_rows(out, out_stride, width, c.q_dtype, "out");
+    if (st == DH_OK) st = check_table_ptrs(t, status);
+    if (st == DH_OK && w.bytes) st = check_device_ptr(ws, "workspace");
+    if (st != DH_OK) return st;
+    const uint64_t eb = dh::dtype_bytes(c.q_dtype);
+    dh::WindowArgs a{};
+    a.t = device_tables(t);
+    a.q = static_cast<const uint8_t*>(q);
+    a.out = static_cast<uint8_t*>(out);
+    a.q_stride = q_stride * eb;
+    a.out_stride = out_stride * eb;
+    a.kv = pool->data;
+    a.scales = pool->scales;
+    a.ws_o = static_cast<float*>(ws);
+    a.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + w.o_bytes);
+    a.hq = c.num_heads;
+    a.hkv = c.num_kv_heads;
+    a.r = r;
+    a.tiled = c.gqa_mapping == DH_GQA_TILED ? 1u : 0u;
+    const float sl = c.scale * 1.4426950408889634f;
+    a.scale_log2 = std::max(fabsf(sl), 0x1p-60f);
+    a.q_sign = sl < 0.f ? (c.q_dtype == DH_DTYPE_F32 ? 0x80000000u : 0x80008000u) : 0u;
+    a.window = int32_t(w.window);
+    a.sinks = int32_t(w.sinks);
+    a.page_limit = pool->num_pages;
+    a.splits = w.splits;
+    a.status = status;
+    hipError_t e = hipError_t(w.wide ? dh::launch_window_wide(a, c.q_dtype, c.kv_format, c.head_dim, stream)
+                                     : dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, stream));
+    if (e != hipSuccess) return fail(DH_EHIP, "window attention launch failed: %s", hipGetErrorString(e));
+    if (w.splits > 1) {
+        e = hipError_t(dh::launch_window_merge(a, c.q_dtype, c.head_dim, stream));
+        if (e != hipSuccess) return fail(DH_EHIP, "merge launch failed: %s", hipGetErrorString(e));
+    }
+    return DH_OK;
+}
+
 /* ------------------------------------------------------------------- merge */
 
 dh_status dh_merge_states(const float* o_a, const float* lse_a, const float* o_b, const float* lse_b,

@@ -215,6 +215,50 @@ struct MergeArgs {
     int32_t* status;
 };
 
+// Device tables of the token operators (dh_token_tables), and what their
+// kernels take.
+struct TokenTables {
+    const int32_t* indices;
+    const int32_t* indptr;
+    const int32_t* kv_len;
+    const int32_t* q_indptr;     // null: one new token a sequence
+    uint32_t batch, num_indices, rows, max_kv_len;
+};
+
+struct TokenCopyArgs {
+    TokenTables t;
+    uint8_t* k;                  // rows: read by append, written by read
+    uint8_t* v;
+    uint64_t k_stride, v_stride; // bytes
+    uint8_t* data;
+    uint8_t* scales;
+    uint32_t num_pages, hkv;
+    int32_t* status;
+};
+
+struct WindowArgs {
+    TokenTables t;
+    const uint8_t* q;
+    uint8_t* out;
+    uint64_t q_stride, out_stride;   // bytes
+    const uint8_t* kv;
+    const uint8_t* scales;
+    float* ws_o;                 // [rows][hq][splits][D] unnormalised O
+    float* ws_ml;                // [rows][hq][splits][2] reference max (log2 units), sum
+    uint32_t hq, hkv, r, tiled;
+    float scale_log2;            // as AttendArgs
+    uint32_t q_sign;
+    int32_t window, sinks;       // window 0: none (sinks then 0)
+    uint32_t page_limit;
+    uint32_t splits;             // >= 1; 1: the attention kernel writes out
+    int32_t* status;
+};
+
+// Query rows of a narrow block (one MFMA tile), and of a wide one; pages a
+// wave of a narrow block and a wide block may be given (registers, LDS list).
+constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256, kWideMaxPages = 2048;
+DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 256 ? 128u : 256u; }
+
 // Byte offset of the (page, plane, kv head) 16 x D block in the pool.
 DH_HOST_DEVICE inline uint64_t plane_offset(uint32_t page, uint32_t plane, uint32_t head,
                                                  uint32_t hkv, uint32_t head_dim,
@@ -272,5 +316,11 @@ constexpr uint32_t kCsrWaveSlots = 2048;
 // with 4 096.
 constexpr uint32_t kCsrExtraGrid = 1024;
 constexpr uint32_t kCsrMinChunk = 1, kCsrMaxChunk = uint32_t(kWaveIdRegs) * 64;
+// Token operators (token_kernels.hip, window_kernels.hip).
+int launch_append_tokens(const TokenCopyArgs& a, uint32_t src_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_read_tokens(const TokenCopyArgs& a, uint32_t dst_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_wide(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 }  // namespace dh
 }

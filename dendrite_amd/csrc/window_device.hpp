@@ -1,0 +1,77 @@
+// Blocks of query rows of the windowed attention kernels: which sequence, KV
+// head and rows a workgroup has, and which pages those rows see.
+//
+// Row rho of a sequence is query head offset rho % r of its new token rho / r
+// (r query heads share a KV head), so the rows of a block cover neighbouring
+// positions and read nearly the same tokens.  A row at position p sees
+// tokens t <= p with t > p - window or t < sinks; a block's pages are those of
+// its sinks that lie before its window, then its window's, one list of
+// `pages` entries.
+#pragma once
+#include "token_device.hpp"
+
+namespace dh {
+namespace {
+
+struct RowBlock {
+    Sequence seq;
+    int rho0, nrows;      // first row, rows (0: the block does not exist)
+    int kv_head;
+    int pmin, pmax;       // positions of the first and the last row
+    int sink_pages;       // list entries before the window's
+    int window_page;      // the window's first page of the table
+    int pages;            // entries of the list
+    bool zero;            // rows of a refused or unused sequence: zeros
+};
+
+// Block `unit` of `kRows` rows (a power of two, 1 << SHIFT), KV head kv_head.
+template <int SHIFT>
+__device__ __forceinline__ RowBlock find_rows(const WindowArgs& a, uint64_t unit, int kv_head) {
+    RowBlock k{};
+    k.kv_head = kv_head;
+    uint32_t b, u;
+    if (a.t.q_indptr) {
+        b = find_sequence(a.t, unit, a.r, SHIFT, 1, u);
+    } else {
+        const uint32_t per = (a.r + (1u << SHIFT) - 1) >> SHIFT;
+        if (unit >= uint64_t(a.t.batch) * per) return k;
+        b = uint32_t(unit) / per;
+        u = uint32_t(unit) - b * per;
+    }
+    k.seq = uniform_sequence(load_sequence(a.t, b));
+    const int64_t rows = int64_t(k.seq.nrows) * a.r, rho0 = int64_t(u) << SHIFT;
+    if (rho0 >= rows) return k;
+    k.rho0 = int(rho0);
+    k.nrows = int(min(int64_t(1) << SHIFT, rows - rho0));
+    k.zero = !k.seq.ok || k.seq.n == 0;
+    if (k.zero) return k;
+    const int first = k.seq.len - k.seq.n;
+    k.pmin = first + k.rho0 / int(a.r);
+    k.pmax = first + (k.rho0 + k.nrows - 1) / int(a.r);
+    const int lo = a.window ? max(0, k.pmin - a.window + 1) : 0;
+    k.window_page = lo >> 4;
+    k.sink_pages = a.window ? min((min(a.sinks, k.pmax + 1) + 15) >> 4, k.window_page) : 0;
+    k.pages = k.sink_pages + (k.pmax >> 4) + 1 - k.window_page;
+    return k;
+}
+
+// Page of the table that list entry j stands for.
+__device__ __forceinline__ int list_page(const RowBlock& k, int j) {
+    return j < k.sink_pages ? j : k.window_page + j - k.sink_pages;
+}
+
+// Row rho's offset (in rows of q / out) and query head.
+__device__ __forceinline__ void row_place(const WindowArgs& a, const RowBlock& k, int rho, int& token, int& head) {
+    token = rho / int(a.r);
+    const int j = rho - token * int(a.r);
+    head = a.tiled ? k.kv_head + j * int(a.hkv) : k.kv_head * int(a.r) + j;
+}
+
+// Blocks of 1 << shift rows the call may need (find_rows' numbering).
+inline uint64_t row_blocks(const WindowArgs& a, int shift) {
+    if (!a.t.q_indptr) return uint64_t(a.t.batch) * ((a.r + (1u << shift) - 1) >> shift);
+    return (uint64_t(a.t.rows) * a.r >> shift) + a.t.batch;
+}
+
+}  // namespace
+}  // namespace dh

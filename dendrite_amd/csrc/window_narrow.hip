@@ -1,0 +1,509 @@
+// Windowed attention of few query rows a sequence, from device tables: single
+// tokens and short chunks (dh_attend_window), and the merge of split work.
+//
+// A workgroup of four waves has one block of 16 rows (one MFMA tile) of one KV
+// head and one of `splits` equal parts of the block's page list; each wave
+// takes a quarter of the part, a pair of pages (32 tokens) at a time, with the
+// loads of the next pair in flight behind the math of the current one:
+//   s = scale q K^T, m' = max(m, max s), O = O 2^(m - m') + 2^(s - m') V,
+//   L = L 2^(m - m') + sum 2^(s - m')   (s in log2 units)
+// with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32 (16x16x4 for
+// f32), operands straight from global memory (attend_device.hpp's layout).
+// The waves' states are joined in LDS; with several parts each workgroup
+// writes (O, m, L) in f32 and window_merge_kernel joins them.  Bound by the
+// cache's bytes: every page is read once per block.
+#include "attend_device.hpp"
+#include "window_device.hpp"
+
+namespace dh {
+namespace {
+
+// The page ids of a wave's part of the list, kNarrowWavePages at most, in
+// registers (lane l holds entries l, l + 64, ...): -1 for an entry outside the
+// pool, whose tokens nobody sees.
+struct WavePages {
+    int id[kNarrowWavePages / 64];
+    int j0, n;      // first list entry, entries
+
+    __device__ __forceinline__ void load(const WindowArgs& a, const RowBlock& k, int part, int parts) {
+        int per = (k.pages + parts - 1) / parts;
+        per += per & 1;
+        j0 = min(part * per, k.pages);
+        n = min(min(per, k.pages - j0), int(kNarrowWavePages));
+        const int lane = threadIdx.x & 63;
+        #pragma unroll
+        for (int i = 0; i < int(kNarrowWavePages / 64); ++i) {
+            const int j = lane + 64 * i;
+            id[i] = -1;
+            if (j < n) id[i] = checked_page(a.t.indices[k.seq.page0 + list_page(k, j0 + j)], a.page_limit, a.status);
+        }
+    }
+    __device__ __forceinline__ int at(int j) const {
+        int r = -1;
+        #pragma unroll
+        for (int i = 0; i < int(kNarrowWavePages / 64); ++i)
+            if ((j >> 6) == i) r = __builtin_amdgcn_readlane(id[i], j & 63);
+        return j < n ? r : -1;
+    }
+};
+
+// Tokens of a page (base token t0) that one row at position p sees.
+struct Sight {
+    int p, lo, sinks;     // t <= p and (t >= lo or t < sinks)
+    __device__ __forceinline__ bool sees(int t) const { return t <= p && (t >= lo || t < sinks); }
+};
+
+__device__ __forceinline__ int window_lo(const WindowArgs& a, int p) { return a.window ? p - a.window + 1 : 0; }
+
+// Whether every row of a block sees all of a page / any row sees any of it.
+__device__ __forceinline__ bool all_see(const WindowArgs& a, int pmin, int pmax, int t0) {
+    return t0 + 15 <= pmin && (t0 >= window_lo(a, pmax) || t0 + 15 < a.sinks);
+}
+
+// Joins the states of the workgroup's four waves and writes the block's rows:
+// to out, or as one part's state to the workspace.  Lane (g, c) holds
+// O[row c][(4g + i) * EPL + e] = O[e][i], L its row's sum (already over the
+// four lanes of the row) and m the row's reference.
+template <int D, uint32_t QT>
+__device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& k, int split, float m, float L,
+                                           const f4 (&O)[D / 16], float* lds) {
+    constexpr int EPL = D / 16, RS = D + 4;          // padded row
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    float* o = lds + wave * 16 * RS;
+    float* ml = lds + kWaves * 16 * RS;              // [wave][16][2]
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4)
+            *reinterpret_cast<f4*>(o + c * RS + (4 * g + i) * EPL + e) = f4{O[e][i], O[e + 1][i], O[e + 2][i], O[e + 3][i]};
+    if (g == 0) {
+        ml[(wave * 16 + c) * 2] = m;
+        ml[(wave * 16 + c) * 2 + 1] = L;
+    }
+    __syncthreads();
+    const int row = tid >> 4, d0 = (tid & 15) * EPL;
+    if (row >= k.nrows) return;
+    float mx = kNegInf;
+    #pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[(w * 16 + row) * 2]);
+    float x[EPL], sum = 0.f;
+    #pragma unroll
+    for (int e = 0; e < EPL; ++e) x[e] = 0.f;
+    #pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float mw = ml[(w * 16 + row) * 2];
+        const float al = mw == kNegInf ? 0.f : fast_exp2(mw - mx);
+        sum += al * ml[(w * 16 + row) * 2 + 1];
+        const f4* p = reinterpret_cast<const f4*>(lds + (w * 16 + row) * RS + d0);
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4) {
+            const f4 v = p[e / 4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) x[e + i] += al * v[i];
+        }
+    }
+    int token, head;
+    row_place(a, k, k.rho0 + row, token, head);
+    const uint64_t at = uint64_t(k.seq.row0) + token;
+    if (a.splits > 1) {
+        const uint64_t slot = (at * a.hq + head) * a.splits + split;
+        f4* p = reinterpret_cast<f4*>(a.ws_o + slot * D + d0);
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4) p[e / 4] = f4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+        if ((tid & 15) == 0) *reinterpret_cast<f2*>(a.ws_ml + slot * 2) = f2{mx, sum};
+        return;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    if constexpr (QT == DH_DTYPE_F32) {
+        f4* p = reinterpret_cast<f4*>(a.out + at * a.out_stride + (uint64_t(head) * D + d0) * 4);
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4) p[e / 4] = f4{x[e] * inv, x[e + 1] * inv, x[e + 2] * inv, x[e + 3] * inv};
+    } else {
+        uint32_t w[EPL / 2];
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 2) w[e / 2] = pack2(x[e] * inv, x[e + 1] * inv, QT == DH_DTYPE_F16);
+        store_u32s<EPL / 2>(reinterpret_cast<uint16_t*>(a.out + at * a.out_stride) + uint64_t(head) * D + d0, w);
+    }
+}
+
+// Zero rows of a refused or unused sequence.
+template <int D, uint32_t QT>
+__device__ __forceinline__ void zero_rows(const WindowArgs& a, const RowBlock& k) {
+    constexpr int EB = QT == DH_DTYPE_F32 ? 4 : 2, W = D * EB / 16;      // 16-byte words a row
+    for (int i = threadIdx.x; i < k.nrows * W; i += blockDim.x) {
+        int token, head;
+        row_place(a, k, k.rho0 + i / W, token, head);
+        reinterpret_cast<u32x4*>(a.out + (uint64_t(k.seq.row0) + token) * a.out_stride + uint64_t(head) * D * EB)[i % W] =
+            u32x4{0u, 0u, 0u, 0u};
+    }
+}
+
+// The block of a workgroup: KV heads fastest (neighbouring pages' planes),
+// then parts, then blocks.
+template <int SHIFT>
+__device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& split) {
+    report_bad_tables(a.t, a.status, blockIdx.x);
+    const uint32_t x = blockIdx.x / a.hkv;
+    const int head = int(blockIdx.x - x * a.hkv);
+    const uint32_t unit = x / a.splits;
+    split = int(x - unit * a.splits);
+    return find_rows<SHIFT>(a, unit, head);
+}
+
+template <int D, uint32_t KVF, bool F16>
+__global__ __launch_bounds__(256) void window_narrow_kernel(WindowArgs a) {
+    using R = PageRaw<D, KVF>;
+    constexpr int KB = D / 32, EPL = D / 16;
+    constexpr uint32_t QT = F16 ? DH_DTYPE_F16 : DH_DTYPE_BF16;
+    __shared__ __attribute__((aligned(16))) float lds[kWaves * 16 * (D + 4) + kWaves * 32];
+    int split;
+    const RowBlock k = workgroup_rows<4>(a, split);
+    if (k.nrows == 0) return;
+    if (k.zero) {
+        if (split == 0 && a.splits == 1) zero_rows<D, QT>(a, k);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
+    WavePages pages;
+    pages.load(a, k, split * kWaves + wave, int(a.splits) * kWaves);
+
+    // Query rows as B operands: lane (g, c) holds row c.
+    const int rho = k.rho0 + min(c, k.nrows - 1);
+    int token, head;
+    row_place(a, k, rho, token, head);
+    uint32_t qB[1][KB][4];
+    {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q + (uint64_t(k.seq.row0) + token) * a.q_stride) +
+                             uint64_t(head) * D;
+        #pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            load_dwords<4>(qB[0][kb], qp + (R::FP8 ? 64 * (kb >> 1) + 16 * g + 8 * (kb & 1) : kb * 32 + 8 * g));
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) qB[0][kb][i] ^= a.q_sign;
+        }
+    }
+    Sight row;
+    row.p = k.seq.len - k.seq.n + token;
+    row.lo = window_lo(a, row.p);
+    row.sinks = a.sinks;
+    const Sight any{k.pmax, window_lo(a, k.pmin), a.sinks};    // what some row of the block sees
+
+    float m = kNegInf;
+    f4 L = {0.f, 0.f, 0.f, 0.f};
+    f4 O[EPL];
+    #pragma unroll
+    for (int e = 0; e < EPL; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
+    AttendArgs kv{};
+    kv.kv = a.kv;
+    kv.scales = a.scales;
+    kv.hkv = a.hkv;
+    const float* bsc = reinterpret_cast<const float*>(a.scales);
+
+    R pr[2];
+    float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+    auto load_k = [&](int pair) {
+        #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int id = pages.at(2 * pair + q);
+            const uint32_t pg = uint32_t(max(id, 0));
+            load_page_k<D, KVF>(pr[q], kv, pg, k.kv_head, g, c);
+            if constexpr (KVF == KVF_FP8) ks[q] = id < 0 ? 1.f : bsc[(uint64_t(pg) * 2 + 0) * a.hkv + k.kv_head];
+        }
+    };
+    auto load_v = [&](int pair) {
+        #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int id = pages.at(2 * pair + q);
+            const uint32_t pg = uint32_t(max(id, 0));
+            load_page_v<D, KVF>(pr[q], kv, pg, k.kv_head, g, c);
+            if constexpr (KVF == KVF_FP8) vs[q] = id < 0 ? 1.f : bsc[(uint64_t(pg) * 2 + 1) * a.hkv + k.kv_head];
+        }
+    };
+    const int npairs = (pages.n + 1) >> 1;
+    if (npairs > 0) {
+        load_k(0);
+        load_v(0);
+    }
+    #pragma unroll 1
+    for (int pi = 0; pi < npairs; ++pi) {
+        const bool refill = pi + 1 < npairs;
+        int t0[2];
+        bool ok[2], full = true;
+        #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            ok[q] = pages.at(2 * pi + q) >= 0;
+            t0[q] = 16 * list_page(k, pages.j0 + 2 * pi + q);
+            full = full && ok[q] && all_see(a, k.pmin, k.pmax, t0[q]);
+        }
+        uint32_t kop[2][KB][4];
+        f4 s[1][2];
+        k_operand<D, KVF, F16>(pr[0], kop[0]);
+        k_operand<D, KVF, F16>(pr[1], kop[1]);
+        pair_scores<D, F16, 1, 1>(kop[0], kop[1], qB, s);
+        // A scale of zero (a page nobody wrote) must not meet a masked -inf.
+        const float f0 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[0], 1e-30f) : a.scale_log2;
+        const float f1 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[1], 1e-30f) : a.scale_log2;
+        const float v0s = vs[0], v1s = vs[1];
+        if (refill) load_k(pi + 1);
+        uint32_t vop[2][4][D / 32];
+        #pragma unroll
+        for (int q = 0; q < 2; ++q)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool keep = full || (ok[q] && any.sees(t0[q] + 4 * g + j));
+                if constexpr (!R::FP8) {
+                    #pragma unroll
+                    for (int w = 0; w < R::VW; ++w) vop[q][j][w] = keep ? pr[q].v[j][w] : 0u;
+                } else {
+                    const float sc = KVF == KVF_MX && keep ? e8m0_to_float(pr[q].vsc[j]) : 1.f;
+                    #pragma unroll
+                    for (int w = 0; w < R::VW; ++w)
+                        e4m3x4_cvt<F16>(keep ? pr[q].v[j][w] : 0u, sc, vop[q][j][2 * w], vop[q][j][2 * w + 1]);
+                }
+            }
+        float x[8];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = s[0][0][i];
+            x[4 + i] = s[0][1][i];
+        }
+        if (!full) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(ok[0] && row.sees(t0[0] + 4 * g + i))) x[i] = kNegInf;
+                if (!(ok[1] && row.sees(t0[1] + 4 * g + i))) x[4 + i] = kNegInf;
+            }
+        }
+        const float r0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), r1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+        const float lm = fmaxf(r0 * f0, r1 * f1);
+        // The reference moves only when a score passes it by 8 (2^8 at most
+        // then), so the accumulators are seldom rescaled.
+        if (__ballot(lm > m + 8.f)) {
+            const float mx = rowgroup_max(lm);
+            const float mnew = mx > m + 8.f ? mx : m;
+            const float alpha = m == kNegInf ? 0.f : fast_exp2(m - mnew);
+            m = mnew;
+            L *= alpha;
+            #pragma unroll
+            for (int e = 0; e < EPL; ++e) O[e] *= alpha;
+        }
+        const float nm = m == kNegInf ? 0.f : -m;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = fast_exp2(__builtin_fmaf(x[i], f0, nm));
+            x[4 + i] = fast_exp2(__builtin_fmaf(x[4 + i], f1, nm));
+        }
+        const uint32_t one2 = F16 ? 0x3C003C00u : 0x3F803F80u;
+        const uint32_t ones[4] = {one2, one2, one2, one2};
+        uint32_t pk[4] = {pack2(x[0], x[1], F16), pack2(x[2], x[3], F16), pack2(x[4], x[5], F16), pack2(x[6], x[7], F16)};
+        L = mma16<F16>(ones, pk, L);        // the sum of the weights as V gets them
+        if constexpr (KVF == KVF_FP8) {
+            pk[0] = pack2(x[0] * v0s, x[1] * v0s, F16);
+            pk[1] = pack2(x[2] * v0s, x[3] * v0s, F16);
+            pk[2] = pack2(x[4] * v1s, x[5] * v1s, F16);
+            pk[3] = pack2(x[6] * v1s, x[7] * v1s, F16);
+        }
+        #pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int w = e >> 1;
+            const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+            const uint32_t vA[4] = {__builtin_amdgcn_perm(vop[0][1][w], vop[0][0][w], sel),
+                                    __builtin_amdgcn_perm(vop[0][3][w], vop[0][2][w], sel),
+                                    __builtin_amdgcn_perm(vop[1][1][w], vop[1][0][w], sel),
+                                    __builtin_amdgcn_perm(vop[1][3][w], vop[1][2][w], sel)};
+            O[e] = mma16<F16>(vA, pk, O[e]);
+        }
+        if (refill) load_v(pi + 1);
+    }
+    join_waves<D, QT>(a, k, split, m, L[0], O, lds);
+}
+
+// f32 queries and cache: one page a step on v_mfma_f32_16x16x4_f32.
+template <int D>
+__global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
+    constexpr int KQ = D / 4, EPL = D / 16;
+    __shared__ __attribute__((aligned(16))) float lds[kWaves * 16 * (D + 4) + kWaves * 32];
+    int split;
+    const RowBlock k = workgroup_rows<4>(a, split);
+    if (k.nrows == 0) return;
+    if (k.zero) {
+        if (split == 0 && a.splits == 1) zero_rows<D, DH_DTYPE_F32>(a, k);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
+    WavePages pages;
+    pages.load(a, k, split * kWaves + wave, int(a.splits) * kWaves);
+    const int rho = k.rho0 + min(c, k.nrows - 1);
+    int token, head;
+    row_place(a, k, rho, token, head);
+    float qv[KQ];
+    load_dwords<KQ>(reinterpret_cast<uint32_t*>(qv),
+                    a.q + (uint64_t(k.seq.row0) + token) * a.q_stride + (uint64_t(head) * D + g * KQ) * 4);
+    #pragma unroll
+    for (int i = 0; i < KQ; ++i) qv[i] = __uint_as_float(__float_as_uint(qv[i]) ^ a.q_sign);
+    Sight row;
+    row.p = k.seq.len - k.seq.n + token;
+    row.lo = window_lo(a, row.p);
+    row.sinks = a.sinks;
+    const Sight any{k.pmax, window_lo(a, k.pmin), a.sinks};
+    float m = kNegInf, l = 0.f;
+    f4 O[EPL];
+    #pragma unroll
+    for (int e = 0; e < EPL; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
+    float kb[KQ], vb[4][EPL];
+    auto load = [&](int j) {
+        const uint8_t* kp = a.kv + plane_offset(uint32_t(max(pages.at(j), 0)), 0, k.kv_head, a.hkv, D, 4);
+        const uint8_t* vp = kp + uint64_t(a.hkv) * (kPageSize * D * 4);
+        load_dwords<KQ>(reinterpret_cast<uint32_t*>(kb), kp + (c * D + g * KQ) * 4);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            load_dwords<EPL>(reinterpret_cast<uint32_t*>(vb[i]), vp + ((4 * g + i) * D + c * EPL) * 4);
+    };
+    if (pages.n > 0) load(0);
+    #pragma unroll 1
+    for (int j = 0; j < pages.n; ++j) {
+        const bool ok = pages.at(j) >= 0;
+        const int t0 = 16 * list_page(k, pages.j0 + j);
+        f4 s = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int i = 0; i < KQ; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[i], qv[i], s, 0, 0, 0);
+        float x[4], mx = kNegInf;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = ok && row.sees(t0 + 4 * g + i) ? s[i] * a.scale_log2 : kNegInf;
+            mx = fmaxf(mx, x[i]);
+        }
+        mx = fmaxf(rowgroup_max(mx), m);
+        const float ref = mx == kNegInf ? 0.f : mx, alpha = fast_exp2(m - ref);
+        m = mx;
+        float ps = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = fast_exp2(x[i] - ref);
+            ps += x[i];
+        }
+        l = l * alpha + ps;
+        #pragma unroll
+        for (int e = 0; e < EPL; ++e) O[e] *= alpha;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool keep = ok && any.sees(t0 + 4 * g + i);
+            #pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(keep ? vb[i][e] : 0.f, x[i], O[e], 0, 0, 0);
+        }
+        if (j + 1 < pages.n) load(j + 1);
+    }
+    join_waves<D, DH_DTYPE_F32>(a, k, split, m, rowgroup_sum(l), O, lds);
+}
+
+// Joins the parts of split work: 16 rows of one KV head a workgroup, 16 lanes
+// a row, blocks as the narrow kernel's.
+template <int D, uint32_t QT>
+__global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
+    constexpr int EPL = D / 16;
+    const uint32_t unit = blockIdx.x / a.hkv;
+    const RowBlock k = find_rows<4>(a, unit, int(blockIdx.x - unit * a.hkv));
+    if (k.nrows == 0) return;
+    if (k.zero) {
+        zero_rows<D, QT>(a, k);
+        return;
+    }
+    const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * EPL;
+    if (row >= k.nrows) return;
+    int token, head;
+    row_place(a, k, k.rho0 + row, token, head);
+    const uint64_t at = uint64_t(k.seq.row0) + token, slot = (at * a.hq + head) * a.splits;
+    const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
+    float mx = kNegInf;
+    for (uint32_t s = 0; s < a.splits; ++s) mx = fmaxf(mx, ml[s][0]);
+    float x[EPL], sum = 0.f;
+    #pragma unroll
+    for (int e = 0; e < EPL; ++e) x[e] = 0.f;
+    #pragma unroll 4
+    for (uint32_t s = 0; s < a.splits; ++s) {
+        const f2 v = ml[s];
+        const float al = v[0] == kNegInf ? 0.f : fast_exp2(v[0] - mx);
+        sum += al * v[1];
+        const f4* p = reinterpret_cast<const f4*>(a.ws_o + (slot + s) * D + d0);
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4) {
+            const f4 o = p[e / 4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) x[e + i] += al * o[i];
+        }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    if constexpr (QT == DH_DTYPE_F32) {
+        f4* p = reinterpret_cast<f4*>(a.out + at * a.out_stride + (uint64_t(head) * D + d0) * 4);
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 4) p[e / 4] = f4{x[e] * inv, x[e + 1] * inv, x[e + 2] * inv, x[e + 3] * inv};
+    } else {
+        uint32_t w[EPL / 2];
+        #pragma unroll
+        for (int e = 0; e < EPL; e += 2) w[e / 2] = pack2(x[e] * inv, x[e + 1] * inv, QT == DH_DTYPE_F16);
+        store_u32s<EPL / 2>(reinterpret_cast<uint16_t*>(a.out + at * a.out_stride) + uint64_t(head) * D + d0, w);
+    }
+}
+
+template <int D>
+hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, dim3 grid, hipStream_t s) {
+    const dim3 block(256);
+    if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32)
+        hipLaunchKernelGGL((window_narrow32_kernel<D>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_BF16)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_F16)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_FP8)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, false>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_FP8)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, true>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_MX)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, false>), grid, block, 0, s, a);
+    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_MX)
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, true>), grid, block, 0, s, a);
+    else
+        return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_merge_w(const WindowArgs& a, uint32_t q_dtype, dim3 grid, hipStream_t s) {
+    switch (q_dtype) {
+        case DH_DTYPE_F16: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_F16>), grid, dim3(256), 0, s, a); break;
+        case DH_DTYPE_BF16: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_BF16>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_F32>), grid, dim3(256), 0, s, a); break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream) {
+    const uint64_t blocks = row_blocks(a, 4) * a.splits * a.hkv;
+    if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    const dim3 grid{uint32_t(blocks)};
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    switch (d) {
+        case 64: return launch_narrow_d<64>(a, q_dtype, fmt, grid, s);
+        case 128: return launch_narrow_d<128>(a, q_dtype, fmt, grid, s);
+        case 256: return launch_narrow_d<256>(a, q_dtype, fmt, grid, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream) {
+    const uint64_t blocks = row_blocks(a, 4) * a.hkv;
+    if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    const dim3 grid{uint32_t(blocks)};
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    switch (d) {
+        case 64: return launch_merge_w<64>(a, q_dtype, grid, s);
+        case 128: return launch_merge_w<128>(a, q_dtype, grid, s);
+        case 256: return launch_merge_w<256>(a, q_dtype, grid, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace dh

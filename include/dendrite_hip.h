@@ -107,9 +107,10 @@ typedef struct dh_attn_config {
     uint32_t head_dim;        /* 64, 128 or 256 (flashinfer/mod.rs:20)         */
     float scale;              /* softmax scale, 1/sqrt(head_dim) by default;
                                  any finite value (0 gives uniform weights)   */
-    uint32_t sliding_window;  /* 0 = None.  Accepted and ignored, as by every
-                                 Dendrite backend (backend.rs:206-265 never
-                                 reads it): attention spans all tokens.       */
+    uint32_t sliding_window;  /* 0 = None.  Read by dh_attend_window; accepted
+                                 and ignored elsewhere, as by every Dendrite
+                                 backend (backend.rs:206-265 never reads it):
+                                 attention there spans all tokens.            */
     uint32_t gqa_mapping;     /* dh_gqa_mapping, DH_GQA_TILED by default       */
     uint32_t q_dtype;         /* dh_dtype of q and out (out dtype = q dtype)   */
     uint32_t kv_format;       /* dh_kv_format of the pool this config reads    */
@@ -480,6 +481,109 @@ dh_status dh_decode_stages(dh_backend* backend, const dh_pool* pool,
                            const int32_t* last_page_len, void* out,
                            void* workspace, size_t workspace_bytes,
                            uint32_t stage_mask, void* stream);
+
+/* ------------------------------------------- token operators, device tables */
+
+/* What a step knows of its sequences, in device memory: where their tokens
+ * are and which of them are new.  Token t of sequence b is slot t % 16 of
+ * page indices[indptr[b] + t / 16] (a table position stands for its tokens,
+ * unlike the page lists of dh_plan_create and dh_decode_csr, from which
+ * INVALID entries are dropped).  The sequence holds kv_len[b] tokens, the new
+ * ones included; its last n = q_indptr[b + 1] - q_indptr[b] tokens are the
+ * call's rows q_indptr[b] .. q_indptr[b + 1] - 1 (q_indptr NULL: one new
+ * token a sequence, row b; kv_len[b] = 0 marks row b as unused).  The arrays
+ * are read on every call, so a captured graph follows them.  The tables of
+ * dendrite-core's PageTable (cache/paged.rs:376-390) plus the lengths.
+ *
+ * The counts are the host's and bound what the device arrays may say.  A
+ * sequence is refused when its indptr entries are not in order within
+ * [0, num_indices], kv_len[b] is negative or above max_kv_len, its table is
+ * shorter than its tokens, its q_indptr entries are not in order within
+ * [0, rows], or it has more new tokens than tokens: nothing is read or
+ * written for it (dh_attend_window zeroes its rows if q_indptr is in order).
+ * A table entry outside the pool that a call needs is skipped: DH_INVALID_PAGE
+ * silently, any other id is an error.  `status` (device int32 or NULL) of the
+ * calls below receives DH_EINVAL in either case and is otherwise left as it
+ * was: clear it once and look at it as often as wanted.  Rows that belong to
+ * no sequence are left as they were. */
+typedef struct dh_token_tables {
+    const int32_t* indices;    /* device int32[num_indices], page ids          */
+    const int32_t* indptr;     /* device int32[batch_size + 1]                 */
+    const int32_t* kv_len;     /* device int32[batch_size]                     */
+    const int32_t* q_indptr;   /* device int32[batch_size + 1] or NULL         */
+    uint32_t batch_size;
+    uint32_t num_indices;
+    uint32_t rows;             /* rows of the call's q / out / k / v           */
+    uint32_t max_kv_len;       /* no sequence holds more tokens; sizes the work */
+} dh_token_tables;
+
+/* Writes the new tokens' K and V into their pages in the pool's format.
+ *   k, v     : device, row i at k + i * k_stride elements of src_dtype
+ *              (DH_DTYPE_*), [num_kv_heads][head_dim] each; strides >=
+ *              num_kv_heads * head_dim, both rows and strides multiples of 16
+ *              bytes (views of a fused projection's output will do).
+ * F32 / BF16 / F16 pools: round to nearest even.  MXFP8: each token's groups
+ * as dh_pool_write_pages_device codes them.  FP8_E4M3, per (page, K|V, head)
+ * block, A the largest finite magnitude the call writes to it:
+ *   - the block's first token is among them: scale = max(A / 448, 2^-64);
+ *   - else the block keeps its scale s if A <= 448 s; otherwise s is doubled
+ *     until that holds, and the codes of the block's earlier tokens are
+ *     halved as often (exact unless they become subnormal);
+ *   element = E4M3 of x / scale, round to nearest even, saturated.
+ * A whole block written at once equals dh_pool_write_pages_device's unless
+ * all of it is below 448 * 2^-64.  NaN elements become NaN codes, infinite
+ * ones saturate; neither moves a scale.  Slots not written keep their
+ * contents.  A page that the call writes must belong to one sequence (after
+ * dh_tree_append_token's copy-on-write it does); the contents of a page
+ * written by two are unspecified.  The device half of
+ * ReferenceBackend::append_kv (attention/backend.rs:285-301) for a batch.
+ * One kernel on `stream`; allocates nothing. */
+dh_status dh_pool_append_tokens(dh_pool* pool, const dh_token_tables* tables, const void* k, const void* v,
+                                uint64_t k_stride, uint64_t v_stride, uint32_t src_dtype, int32_t* status,
+                                void* stream);
+
+/* Reads tokens back: the last n of each sequence (q_indptr - all of them
+ * where n = kv_len) into rows k, v (device, laid out as for
+ * dh_pool_append_tokens) as elements of dst_dtype: code * scale in f32, rounded
+ * to it.
+ * Tokens whose page is outside the pool give zeros.  The device counterpart
+ * of ReferenceBackend::get_kv (attention/backend.rs:135-138), which
+ * dh_pool_read_page leaves coded.  One kernel on `stream`; allocates nothing. */
+dh_status dh_pool_read_tokens(const dh_pool* pool, const dh_token_tables* tables, void* k, void* v,
+                              uint64_t k_stride, uint64_t v_stride, uint32_t dst_dtype, int32_t* status,
+                              void* stream);
+
+/* Workspace bytes of dh_attend_window (0: none needed), from the counts of
+ * `tables` and whether q_indptr is NULL; its arrays are not read. */
+size_t dh_window_workspace_size(const dh_attn_config* cfg, const dh_token_tables* tables, uint32_t sinks);
+
+/* Causal attention of the new tokens over their sequences' pages, with
+ * cfg->sliding_window honoured: the token at position p sees the tokens
+ * t <= p with t > p - sliding_window or t < sinks (sliding_window 0: every
+ * t <= p; sinks then has no effect).  out[i][h] = softmax(scale q[i][h] K^T) V
+ * over them, GQA per cfg->gqa_mapping; a row that sees nothing (pages outside
+ * the pool) is zeros.  Only table entries that some row sees are read, so the
+ * pages between the sinks and the window may be freed and their entries
+ * DH_INVALID_PAGE.  The K / V of the new tokens are expected in the pages
+ * (dh_pool_append_tokens before).  Slots past kv_len may hold anything; a NaN
+ * or infinity among a sequence's own V reaches the rows that see it and may
+ * reach the sequence's other rows of the call.
+ *   q, out    : device, row i at q + i * q_stride elements of cfg->q_dtype,
+ *               [num_heads][head_dim] each; strides >= num_heads * head_dim,
+ *               rows and strides multiples of 16 bytes; out overlaps nothing
+ *               the call reads.
+ *   workspace : device, 256-byte aligned, >= dh_window_workspace_size bytes,
+ *               or NULL if that is 0; holds nothing between calls.  Calls that
+ *               may overlap need one each.
+ * The single-token form (q_indptr NULL) and short chunks are split along the
+ * sequence; long chunks take tiles of query rows.  One kernel on `stream`, two
+ * when the work is split; allocates nothing.  The window that
+ * AttentionConfig::with_sliding_window sets (attention/backend.rs:26-28,44-47)
+ * and no backend reads. */
+dh_status dh_attend_window(dh_backend* backend, const dh_pool* pool, const dh_attn_config* cfg, uint32_t sinks,
+                           const dh_token_tables* tables, const void* q, uint64_t q_stride, void* out,
+                           uint64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,
+                           void* stream);
 
 /* ------------------------------------------------------------------- merge */
 
