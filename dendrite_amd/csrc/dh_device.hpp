@@ -256,8 +256,8 @@ struct WindowArgs {
 
 // Query rows of a narrow block (one MFMA tile), and of a wide one; pages a
 // wave of a narrow block and a wide block may be given (registers, LDS list).
-constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256, kWideMaxPages = 2048;
-DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 256 ? 128u : 256u; }
+constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256, kWideMaxPages = 1024;
+DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 128 ? 256u : 128u; }
 
 // Byte offset of the (page, plane, kv head) 16 x D block in the pool.
 DH_HOST_DEVICE inline uint64_t plane_offset(uint32_t page, uint32_t plane, uint32_t head,

@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t find_sequence(const TokenTables& t, uint64_t
         if (step == 1) break;
         n = min(step, t.batch - lo);
     }
-    unit = u >= base && u - base < 0xFFFFFFFFull ? uint32_t(u - base) : 0xFFFFFFFFu;
+    unit = uint32_t(uniform(int(u >= base && u - base < 0xFFFFFFFFull ? uint32_t(u - base) : 0xFFFFFFFFu)));
     return uint32_t(uniform(int(lo)));
 }
 

@@ -55,6 +55,24 @@ __device__ __forceinline__ RowBlock find_rows(const WindowArgs& a, uint64_t unit
     return k;
 }
 
+// The same, told to the compiler as wave-uniform once more: the fields merge
+// over find_rows' early returns, after which it holds them in vector registers
+// and masks execution where a scalar branch will do.
+__device__ __forceinline__ RowBlock uniform_block(const RowBlock& x) {
+    RowBlock k;
+    k.seq = uniform_sequence(x.seq);
+    k.rho0 = uniform(x.rho0);
+    k.nrows = uniform(x.nrows);
+    k.kv_head = uniform(x.kv_head);
+    k.pmin = uniform(x.pmin);
+    k.pmax = uniform(x.pmax);
+    k.sink_pages = uniform(x.sink_pages);
+    k.window_page = uniform(x.window_page);
+    k.pages = uniform(x.pages);
+    k.zero = uniform(x.zero ? 1 : 0) != 0;
+    return k;
+}
+
 // Page of the table that list entry j stands for.
 __device__ __forceinline__ int list_page(const RowBlock& k, int j) {
     return j < k.sink_pages ? j : k.window_page + j - k.sink_pages;

@@ -26,7 +26,7 @@ struct WavePages {
     int j0, n;      // first list entry, entries
 
     __device__ __forceinline__ void load(const WindowArgs& a, const RowBlock& k, int part, int parts) {
-        int per = (k.pages + parts - 1) / parts;
+        int per = uniform((k.pages + parts - 1) / parts);
         per += per & 1;
         j0 = min(part * per, k.pages);
         n = min(min(per, k.pages - j0), int(kNarrowWavePages));
@@ -144,10 +144,10 @@ template <int SHIFT>
 __device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& split) {
     report_bad_tables(a.t, a.status, blockIdx.x);
     const uint32_t x = blockIdx.x / a.hkv;
-    const int head = int(blockIdx.x - x * a.hkv);
+    const int head = uniform(int(blockIdx.x - x * a.hkv));
     const uint32_t unit = x / a.splits;
-    split = int(x - unit * a.splits);
-    return find_rows<SHIFT>(a, unit, head);
+    split = uniform(int(x - unit * a.splits));
+    return uniform_block(find_rows<SHIFT>(a, unit, head));
 }
 
 template <int D, uint32_t KVF, bool F16>
@@ -397,53 +397,60 @@ __global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
     join_waves<D, DH_DTYPE_F32>(a, k, split, m, rowgroup_sum(l), O, lds);
 }
 
-// Joins the parts of split work: 16 rows of one KV head a workgroup, 16 lanes
-// a row, blocks as the narrow kernel's.
+// Joins the parts of split work, one row a workgroup: D / 4 lanes take a part's
+// O (four elements each), the workgroup's 1024 / D lane groups every so many
+// parts; their sums are added in LDS in a fixed order.
 template <int D, uint32_t QT>
 __global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
-    constexpr int EPL = D / 16;
-    const uint32_t unit = blockIdx.x / a.hkv;
-    const RowBlock k = find_rows<4>(a, unit, int(blockIdx.x - unit * a.hkv));
-    if (k.nrows == 0) return;
-    if (k.zero) {
-        zero_rows<D, QT>(a, k);
-        return;
-    }
-    const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * EPL;
+    constexpr int LPP = D / 4, G = 256 / LPP;
+    __shared__ float red[4];
+    __shared__ __attribute__((aligned(16))) f4 acc[G][LPP];
+    __shared__ float sums[G];
+    const uint32_t x0 = blockIdx.x >> 4, unit = x0 / a.hkv;
+    const int row = int(blockIdx.x & 15);
+    const RowBlock k = find_rows<4>(a, unit, int(x0 - unit * a.hkv));
     if (row >= k.nrows) return;
+    const int tid = threadIdx.x;
     int token, head;
     row_place(a, k, k.rho0 + row, token, head);
     const uint64_t at = uint64_t(k.seq.row0) + token, slot = (at * a.hq + head) * a.splits;
     const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
+    const int splits = k.zero ? 0 : int(a.splits);
     float mx = kNegInf;
-    for (uint32_t s = 0; s < a.splits; ++s) mx = fmaxf(mx, ml[s][0]);
-    float x[EPL], sum = 0.f;
+    for (int s = tid; s < splits; s += 256) mx = fmaxf(mx, ml[s][0]);
     #pragma unroll
-    for (int e = 0; e < EPL; ++e) x[e] = 0.f;
+    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int grp = tid / LPP, col = tid % LPP;
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
     #pragma unroll 4
-    for (uint32_t s = 0; s < a.splits; ++s) {
+    for (int s = grp; s < splits; s += G) {
         const f2 v = ml[s];
         const float al = v[0] == kNegInf ? 0.f : fast_exp2(v[0] - mx);
         sum += al * v[1];
-        const f4* p = reinterpret_cast<const f4*>(a.ws_o + (slot + s) * D + d0);
-        #pragma unroll
-        for (int e = 0; e < EPL; e += 4) {
-            const f4 o = p[e / 4];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) x[e + i] += al * o[i];
-        }
+        x += reinterpret_cast<const f4*>(a.ws_o + (slot + s) * D)[col] * al;
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    if constexpr (QT == DH_DTYPE_F32) {
-        f4* p = reinterpret_cast<f4*>(a.out + at * a.out_stride + (uint64_t(head) * D + d0) * 4);
-        #pragma unroll
-        for (int e = 0; e < EPL; e += 4) p[e / 4] = f4{x[e] * inv, x[e + 1] * inv, x[e + 2] * inv, x[e + 3] * inv};
-    } else {
-        uint32_t w[EPL / 2];
-        #pragma unroll
-        for (int e = 0; e < EPL; e += 2) w[e / 2] = pack2(x[e] * inv, x[e + 1] * inv, QT == DH_DTYPE_F16);
-        store_u32s<EPL / 2>(reinterpret_cast<uint16_t*>(a.out + at * a.out_stride) + uint64_t(head) * D + d0, w);
+    acc[grp][col] = x;
+    if (col == 0) sums[grp] = sum;
+    __syncthreads();
+    if (tid >= LPP) return;
+    x = acc[0][col];
+    sum = sums[0];
+    #pragma unroll
+    for (int g = 1; g < G; ++g) {
+        x += acc[g][col];
+        sum += sums[g];
     }
+    const f4 o = x * (sum > 0.f ? 1.f / sum : 0.f);
+    uint8_t* dst = a.out + at * a.out_stride;
+    if constexpr (QT == DH_DTYPE_F32)
+        *reinterpret_cast<f4*>(dst + (uint64_t(head) * D + 4 * col) * 4) = o;
+    else
+        *reinterpret_cast<u32x2*>(dst + (uint64_t(head) * D + 4 * col) * 2) =
+            u32x2{pack2(o[0], o[1], QT == DH_DTYPE_F16), pack2(o[2], o[3], QT == DH_DTYPE_F16)};
 }
 
 template <int D>
@@ -494,7 +501,7 @@ int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, ui
 }
 
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream) {
-    const uint64_t blocks = row_blocks(a, 4) * a.hkv;
+    const uint64_t blocks = row_blocks(a, 4) * a.hkv * 16;
     if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
     const dim3 grid{uint32_t(blocks)};
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
