@@ -50,7 +50,7 @@ SAN_BUILD = os.path.join(PKG, "_build_san")
 SAN_LIB = os.path.join(SAN_BUILD, "libdendrite_hip.so")
 
 HIP_SOURCES = ["decode_kernels.hip", "csr_kernels.hip", "write_kernels.hip", "token_kernels.hip",
-               "window_narrow.hip", "window_wide.hip"]
+               "window_narrow.hip", "window_wide.hip", "window_ring.hip"]
 HOST_SOURCES = ["api.cpp", "planner.cpp", "block_model.cpp"]
 TESTDATA_SOURCES = ["synth.cpp"]
 

@@ -1341,11 +1341,35 @@ dh_status token_copy(const dh_pool* p, const dh_token_tables* t, const void* k, 
 // How dh_attend_window runs a call: from counts the host has, so the
 // workspace is sized by the same rule.
 struct WindowPlan {
-    bool wide;
+    bool wide, ring;           // query rows in wide blocks; pages straight to LDS
     uint32_t splits;
     uint32_t window, sinks;
     size_t o_bytes, bytes;     // workspace: O, all
 };
+
+// Parts of a wide block's page list: the fewest microseconds by a model of the
+// wide kernels, fitted to their times.  A full chip takes head_dim / 256 us a
+// page of every block, three quarters of that half full, and 14 pages' time to
+// start; a last round that does not fill it counts half empty; the parts' states are written and read at 4.5 TB/s, 4 us the launch.
+// (Tokens x heads of 128 over a 16-bit context, in one part and as chosen: 256 x
+// 64 over a window of 2048 55 and 46 us; 400 x 32 over 12000 134 and 97; 1100 x
+// 32 284 and 243.)
+uint32_t wide_splits(const dh_attn_config& c, bool ring, uint64_t states, uint64_t blocks, uint64_t pages,
+                     uint64_t least) {
+    const double slots = c.head_dim == 256 ? 256 : ring && c.head_dim == 64 ? 768 : 512;
+    const double page = c.head_dim / 256.0, state = states * c.head_dim * 8 / 4.5e6;
+    const uint64_t most = std::max(least, std::min<uint64_t>(pages / 16, uint64_t(2 * slots) / blocks + 1));
+    uint64_t best = least;
+    double low = 0;
+    for (uint64_t s = least; s <= most; ++s) {
+        const double full = blocks * s / slots, rounds = full <= 0.5 ? 0.75 : full <= 1 ? 1 : (full + std::ceil(full)) / 2;
+        const double us = rounds * page * double((pages + s - 1) / s + 14) + (s > 1 ? 4 + s * state : 0);
+        if (s > least && us >= low) continue;
+        best = s;
+        low = us;
+    }
+    return uint32_t(best);
+}
 
 WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32_t sinks) {
     WindowPlan w{};
@@ -1356,17 +1380,27 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     // Wide blocks (256 or 128 rows) where the sequences fill a good part of
     // one, narrow ones (16 rows, each reading the cache by itself) below.
     w.wide = t.q_indptr && c.q_dtype != DH_DTYPE_F32 && rows >= 64 * uint64_t(t.batch_size);
-    const uint64_t block = w.wide ? dh::wide_rows(c.head_dim) : dh::kNarrowRows;
+    // 16-bit caches go straight to LDS; at head_dim 256 that holds 64 rows a
+    // workgroup only, and 128 rows fed through registers are faster (4096 tokens
+    // x 16 heads over 2048: 211 us against 276).
+    w.ring = w.wide && c.head_dim <= 128 && c.kv_format != DH_KV_FP8_E4M3 && c.kv_format != DH_KV_MXFP8;
+    const uint64_t block = !w.wide ? dh::kNarrowRows : w.ring ? dh::kRingRows : dh::wide_rows(c.head_dim);
     const uint64_t all = (uint64_t(t.max_kv_len) + 15) / 16;
     const uint64_t tokens = (block + r - 2) / r + 1;      // most positions a block covers
     const uint64_t pages = w.window ? std::min(all, (w.sinks + 15) / 16 + (w.window + tokens + 14) / 16 + 1) : all;
     const uint64_t blocks = (t.q_indptr ? rows / block + t.batch_size : t.batch_size * ((r + block - 1) / block)) *
                             c.num_kv_heads;
-    const uint64_t cap = w.wide ? dh::kWideMaxPages - 8 : dh::kWaves * (dh::kNarrowWavePages - 2);
+    const uint64_t cap = !w.wide ? dh::kWaves * (dh::kNarrowWavePages - 2)
+                                 : (w.ring ? dh::kRingMaxPages : dh::kWideMaxPages) - 8;
     const uint64_t least = std::max<uint64_t>(1, (pages + cap - 1) / cap);
-    const uint64_t want = (w.wide ? 256u : 512u) / std::max<uint64_t>(1, blocks);
-    const uint64_t most = pages / (w.wide ? 32 : 16);     // a part worth its own state
-    w.splits = uint32_t(std::max(least, std::min(want, most)));
+    if (w.wide) {
+        // blocks that have rows: one a sequence may be part empty
+        const uint64_t filled = (rows + t.batch_size * block / 2 + block / 2 - 1) / block * c.num_kv_heads;
+        w.splits = wide_splits(c, w.ring, uint64_t(t.rows) * c.num_heads, filled, pages, least);
+    } else {
+        const uint64_t want = 512u / std::max<uint64_t>(1, blocks);
+        w.splits = uint32_t(std::max(least, std::min(want, pages / 16)));
+    }
     if (w.splits > 1) {
         const size_t states = size_t(t.rows) * c.num_heads * w.splits;
         w.o_bytes = align256(states * c.head_dim * sizeof(float));
@@ -1442,8 +1476,10 @@ dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_co
     a.page_limit = pool->num_pages;
     a.splits = w.splits;
     a.status = status;
-    hipError_t e = hipError_t(w.wide ? dh::launch_window_wide(a, c.q_dtype, c.kv_format, c.head_dim, stream)
-                                     : dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, stream));
+    hipError_t e = hipError_t(
+        !w.wide  ? dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, stream)
+        : w.ring ? dh::launch_window_ring(a, c.q_dtype, c.head_dim, stream)
+                 : dh::launch_window_wide(a, c.q_dtype, c.kv_format, c.head_dim, stream));
     if (e != hipSuccess) return fail(DH_EHIP, "window attention launch failed: %s", hipGetErrorString(e));
     if (w.splits > 1) {
         e = hipError_t(dh::launch_window_merge(a, c.q_dtype, c.head_dim, stream));

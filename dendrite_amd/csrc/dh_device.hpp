@@ -254,10 +254,17 @@ struct WindowArgs {
     int32_t* status;
 };
 
-// Query rows of a narrow block (one MFMA tile), and of a wide one; pages a
-// wave of a narrow block and a wide block may be given (registers, LDS list).
-constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256, kWideMaxPages = 1024;
-DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 128 ? 256u : 128u; }
+// Query rows of a narrow block (one MFMA tile), of a wide one fed through LDS
+// directly (window_ring.hip) and of one fed through registers; pages a wave of
+// a narrow block and a wide block may be given (registers, LDS lists).
+constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256;
+constexpr int kRingShift = 7;
+constexpr uint32_t kRingRows = 1u << kRingShift, kRingMaxPages = 2048, kWideMaxPages = 384;
+// Parts that are merged 16 rows a workgroup; more are merged one row a
+// workgroup (16384 rows in 3 parts: 5 us against 26; 32 rows in 31: 12 against
+// 4; 2048 in 15: 8.5 against 6).
+constexpr uint32_t kMergeFew = 8;
+DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 64 ? 256u : 128u; }
 
 // Byte offset of the (page, plane, kv head) 16 x D block in the pool.
 DH_HOST_DEVICE inline uint64_t plane_offset(uint32_t page, uint32_t plane, uint32_t head,
@@ -321,6 +328,7 @@ int launch_append_tokens(const TokenCopyArgs& a, uint32_t src_dtype, uint32_t fm
 int launch_read_tokens(const TokenCopyArgs& a, uint32_t dst_dtype, uint32_t fmt, uint32_t d, void* stream);
 int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
 int launch_window_wide(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_ring(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 }  // namespace dh
 }

@@ -85,6 +85,19 @@ __device__ __forceinline__ void row_place(const WindowArgs& a, const RowBlock& k
     head = a.tiled ? k.kv_head + j * int(a.hkv) : k.kv_head * int(a.r) + j;
 }
 
+// Zero rows of a refused or unused sequence.
+typedef uint32_t word16 __attribute__((ext_vector_type(4)));
+template <int D, uint32_t QT>
+__device__ __forceinline__ void zero_rows(const WindowArgs& a, const RowBlock& k) {
+    constexpr int EB = QT == DH_DTYPE_F32 ? 4 : 2, W = D * EB / 16;      // 16-byte words a row
+    for (int i = threadIdx.x; i < k.nrows * W; i += blockDim.x) {
+        int token, head;
+        row_place(a, k, k.rho0 + i / W, token, head);
+        reinterpret_cast<word16*>(a.out + (uint64_t(k.seq.row0) + token) * a.out_stride + uint64_t(head) * D * EB)[i % W] =
+            word16{0u, 0u, 0u, 0u};
+    }
+}
+
 // Blocks of 1 << shift rows the call may need (find_rows' numbering).
 inline uint64_t row_blocks(const WindowArgs& a, int shift) {
     if (!a.t.q_indptr) return uint64_t(a.t.batch) * ((a.r + (1u << shift) - 1) >> shift);

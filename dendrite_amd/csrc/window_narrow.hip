@@ -126,18 +126,6 @@ __device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& 
     }
 }
 
-// Zero rows of a refused or unused sequence.
-template <int D, uint32_t QT>
-__device__ __forceinline__ void zero_rows(const WindowArgs& a, const RowBlock& k) {
-    constexpr int EB = QT == DH_DTYPE_F32 ? 4 : 2, W = D * EB / 16;      // 16-byte words a row
-    for (int i = threadIdx.x; i < k.nrows * W; i += blockDim.x) {
-        int token, head;
-        row_place(a, k, k.rho0 + i / W, token, head);
-        reinterpret_cast<u32x4*>(a.out + (uint64_t(k.seq.row0) + token) * a.out_stride + uint64_t(head) * D * EB)[i % W] =
-            u32x4{0u, 0u, 0u, 0u};
-    }
-}
-
 // The block of a workgroup: KV heads fastest (neighbouring pages' planes),
 // then parts, then blocks.
 template <int SHIFT>
@@ -397,7 +385,50 @@ __global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
     join_waves<D, DH_DTYPE_F32>(a, k, split, m, rowgroup_sum(l), O, lds);
 }
 
-// Joins the parts of split work, one row a workgroup: D / 4 lanes take a part's
+// Writes elements 4 col .. 4 col + 3 of a merged row.
+template <int D, uint32_t QT>
+__device__ __forceinline__ void write_merged(const WindowArgs& a, uint64_t at, int head, int col, f4 x, float sum) {
+    const f4 o = x * (sum > 0.f ? 1.f / sum : 0.f);
+    uint8_t* dst = a.out + at * a.out_stride;
+    if constexpr (QT == DH_DTYPE_F32)
+        *reinterpret_cast<f4*>(dst + (uint64_t(head) * D + 4 * col) * 4) = o;
+    else
+        *reinterpret_cast<u32x2*>(dst + (uint64_t(head) * D + 4 * col) * 2) =
+            u32x2{pack2(o[0], o[1], QT == DH_DTYPE_F16), pack2(o[2], o[3], QT == DH_DTYPE_F16)};
+}
+
+// Joins a few parts of split work (kMergeFew at most), a block of 16 rows a
+// workgroup: D / 4 lanes take a row, four elements each.  Bound by the states'
+// bytes.
+template <int D, uint32_t QT>
+__global__ __launch_bounds__(256) void window_merge_few_kernel(WindowArgs a) {
+    constexpr int LPP = D / 4, G = 256 / LPP;
+    const uint32_t unit = blockIdx.x / a.hkv;
+    const RowBlock k = find_rows<4>(a, unit, int(blockIdx.x - unit * a.hkv));
+    const int grp = threadIdx.x / LPP, col = threadIdx.x % LPP;
+    const int splits = k.zero ? 0 : int(a.splits);
+    #pragma unroll 1
+    for (int row = grp; row < k.nrows; row += G) {
+        int token, head;
+        row_place(a, k, k.rho0 + row, token, head);
+        const uint64_t at = uint64_t(k.seq.row0) + token, slot = (at * a.hq + head) * a.splits;
+        const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
+        const f4* o = reinterpret_cast<const f4*>(a.ws_o + slot * D) + col;
+        float mx = kNegInf, sum = 0.f;
+        for (int s = 0; s < splits; ++s) mx = fmaxf(mx, ml[s][0]);
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const f2 v = ml[s];
+            const float al = v[0] == kNegInf ? 0.f : fast_exp2(v[0] - mx);
+            sum += al * v[1];
+            x += o[s * LPP] * al;
+        }
+        write_merged<D, QT>(a, at, head, col, x, sum);
+    }
+}
+
+// Joins many parts of split work, one row a workgroup: D / 4 lanes take a part's
 // O (four elements each), the workgroup's 1024 / D lane groups every so many
 // parts; their sums are added in LDS in a fixed order.
 template <int D, uint32_t QT>
@@ -444,13 +475,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
         x += acc[g][col];
         sum += sums[g];
     }
-    const f4 o = x * (sum > 0.f ? 1.f / sum : 0.f);
-    uint8_t* dst = a.out + at * a.out_stride;
-    if constexpr (QT == DH_DTYPE_F32)
-        *reinterpret_cast<f4*>(dst + (uint64_t(head) * D + 4 * col) * 4) = o;
-    else
-        *reinterpret_cast<u32x2*>(dst + (uint64_t(head) * D + 4 * col) * 2) =
-            u32x2{pack2(o[0], o[1], QT == DH_DTYPE_F16), pack2(o[2], o[3], QT == DH_DTYPE_F16)};
+    write_merged<D, QT>(a, at, head, col, x, sum);
 }
 
 template <int D>
@@ -475,12 +500,20 @@ hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, 
     return hipGetLastError();
 }
 
+template <int D, uint32_t QT>
+void launch_merge_q(const WindowArgs& a, uint32_t blocks, hipStream_t s) {
+    if (a.splits <= kMergeFew)
+        hipLaunchKernelGGL((window_merge_few_kernel<D, QT>), dim3(blocks), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((window_merge_kernel<D, QT>), dim3(blocks * 16), dim3(256), 0, s, a);
+}
+
 template <int D>
-hipError_t launch_merge_w(const WindowArgs& a, uint32_t q_dtype, dim3 grid, hipStream_t s) {
+hipError_t launch_merge_w(const WindowArgs& a, uint32_t q_dtype, uint32_t blocks, hipStream_t s) {
     switch (q_dtype) {
-        case DH_DTYPE_F16: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_F16>), grid, dim3(256), 0, s, a); break;
-        case DH_DTYPE_BF16: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_BF16>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((window_merge_kernel<D, DH_DTYPE_F32>), grid, dim3(256), 0, s, a); break;
+        case DH_DTYPE_F16: launch_merge_q<D, DH_DTYPE_F16>(a, blocks, s); break;
+        case DH_DTYPE_BF16: launch_merge_q<D, DH_DTYPE_BF16>(a, blocks, s); break;
+        default: launch_merge_q<D, DH_DTYPE_F32>(a, blocks, s); break;
     }
     return hipGetLastError();
 }
@@ -501,9 +534,9 @@ int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, ui
 }
 
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream) {
-    const uint64_t blocks = row_blocks(a, 4) * a.hkv * 16;
-    if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    const dim3 grid{uint32_t(blocks)};
+    const uint64_t blocks = row_blocks(a, 4) * a.hkv;
+    if (blocks > 0x7FFFFFFull) return hipErrorInvalidValue;
+    const uint32_t grid = uint32_t(blocks);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (d) {
         case 64: return launch_merge_w<64>(a, q_dtype, grid, s);
