@@ -1378,12 +1378,19 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     w.window = c.sliding_window >= t.max_kv_len ? 0u : c.sliding_window;
     w.sinks = w.window ? std::min(sinks, t.max_kv_len) : 0u;
     // Wide blocks (256 or 128 rows) where the sequences fill a good part of
-    // one, narrow ones (16 rows, each reading the cache by itself) below.
-    w.wide = t.q_indptr && c.q_dtype != DH_DTYPE_F32 && rows >= 64 * uint64_t(t.batch_size);
+    // one, narrow ones (16 rows, each reading the cache by itself) below.  The
+    // two meet at 24 to 40 rows a sequence (32 sequences over a window of 2001,
+    // narrow and wide: heads of 128, 32 rows, bf16 72 and 60 us, FP8 65 and 54;
+    // 24 rows 53 and 58, 44 and 54), but later where a wide block is dear: 256
+    // rows of 8-bit caches of 64 dims (56 rows in FP8: 39 and 47), one
+    // workgroup a CU at 256 dims (48 rows: 64 and 77 in bf16, 55 and 73 in FP8).
+    const bool codes = c.kv_format == DH_KV_FP8_E4M3 || c.kv_format == DH_KV_MXFP8;
+    const uint64_t fill = c.head_dim == 256 || (codes && c.head_dim == 64) ? 64 : 32;
+    w.wide = t.q_indptr && c.q_dtype != DH_DTYPE_F32 && rows >= fill * t.batch_size;
     // 16-bit caches go straight to LDS; at head_dim 256 that holds 64 rows a
     // workgroup only, and 128 rows fed through registers are faster (4096 tokens
     // x 16 heads over 2048: 211 us against 276).
-    w.ring = w.wide && c.head_dim <= 128 && c.kv_format != DH_KV_FP8_E4M3 && c.kv_format != DH_KV_MXFP8;
+    w.ring = w.wide && c.head_dim <= 128 && !codes;
     const uint64_t block = !w.wide ? dh::kNarrowRows : w.ring ? dh::kRingRows : dh::wide_rows(c.head_dim);
     const uint64_t all = (uint64_t(t.max_kv_len) + 15) / 16;
     const uint64_t tokens = (block + r - 2) / r + 1;      // most positions a block covers

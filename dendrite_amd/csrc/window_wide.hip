@@ -229,15 +229,17 @@ __device__ __forceinline__ void wide_scale(f16v& O, float alpha) {
     if constexpr (ACC) {
         #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            float x = O[i], y = O[i + 1], z = O[i + 2], v = O[i + 3], t;
-            asm volatile("s_nop 15\n\ts_nop 7\n\t"
-                         "v_accvgpr_read_b32 %4, %0\n\ts_nop 0\n\tv_mul_f32 %4, %4, %5\n\ts_nop 0\n\tv_accvgpr_write_b32 %0, %4\n\t"
-                         "v_accvgpr_read_b32 %4, %1\n\ts_nop 0\n\tv_mul_f32 %4, %4, %5\n\ts_nop 0\n\tv_accvgpr_write_b32 %1, %4\n\t"
-                         "v_accvgpr_read_b32 %4, %2\n\ts_nop 0\n\tv_mul_f32 %4, %4, %5\n\ts_nop 0\n\tv_accvgpr_write_b32 %2, %4\n\t"
-                         "v_accvgpr_read_b32 %4, %3\n\ts_nop 0\n\tv_mul_f32 %4, %4, %5\n\ts_nop 0\n\tv_accvgpr_write_b32 %3, %4\n\t"
-                         "s_nop 7"
-                         : "+a"(x), "+a"(y), "+a"(z), "+a"(v), "=&v"(t)
-                         : "v"(alpha));
+            float x = O[i], y = O[i + 1], z = O[i + 2], v = O[i + 3], t0, t1, t2, t3;
+            asm volatile("s_nop %9\n\ts_nop %9\n\t"
+                         "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+                         "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\t"
+                         "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
+                         "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
+                         "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+                         "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\t"
+                         "s_nop %10"
+                         : "+a"(x), "+a"(y), "+a"(z), "+a"(v), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+                         : "v"(alpha), "i"(i == 0 ? 15 : 0), "i"(i == 12 ? 7 : 0));
             O[i] = x;
             O[i + 1] = y;
             O[i + 2] = z;
