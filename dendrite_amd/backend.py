@@ -29,10 +29,23 @@ def _torch():
     return torch
 
 
+_CODES: dict = {}      # torch dtype -> dh_dtype, filled on first use
+
+
 def dtype_code(t) -> int:
-    torch = _torch()
-    return {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16,
-            torch.float32: _lib.DTYPE_F32}[t]
+    if not _CODES:
+        torch = _torch()
+        _CODES.update({torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16,
+                       torch.float32: _lib.DTYPE_F32})
+    return _CODES[t]
+
+
+def _code(t) -> Optional[int]:
+    """dtype_code of a tensor, None where it has none."""
+    try:
+        return dtype_code(t.dtype)
+    except KeyError:
+        return None
 
 
 def torch_dtype(code: int):
@@ -75,28 +88,39 @@ def _stream_ptr(stream) -> Optional[int]:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+_raw_stream = None     # device index -> hipStream_t of torch's current stream
+
+
 def _device_stream(stream, device: int) -> Optional[int]:
     """The hipStream_t of `stream`; None: torch's current stream on `device`,
     whichever device is current."""
+    global _raw_stream
     if stream is None:
-        return _torch().cuda.current_stream(device).cuda_stream
+        if _raw_stream is None:
+            torch = _torch()
+            # (a stream object costs a microsecond to make)
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                  lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return _raw_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _on_device(t, device: int, what: str) -> None:
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise DhError(_lib.DH_EINVAL, f"{what} is on {t.device}, not on cuda:{device}")
 
 
 def _rows(t, heads: int, dim: int, device: int, what: str) -> int:
     """Checks rows [n, heads, dim] whose elements lie together in each row;
     returns the row stride in elements."""
-    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, dim):
-        raise DhError(_lib.DH_EINVAL, f"{what} shape {tuple(t.shape)} is not [rows, {heads}, {dim}]")
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise DhError(_lib.DH_EINVAL, f"{what} shape {tuple(shape)} is not [rows, {heads}, {dim}]")
     _on_device(t, device, what)
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (heads > 1 and s1 != dim):
         raise DhError(_lib.DH_EINVAL, f"{what}: the elements of a row must be contiguous (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+    return s0 if shape[0] > 1 else heads * dim
 
 
 class TokenTables:
@@ -135,18 +159,22 @@ class TokenTables:
         c.q_indptr = None if q_indptr is None else q_indptr.data_ptr()
         c.batch_size, c.num_indices, c.max_kv_len = self.batch_size, indices.numel(), self.max_kv_len
         self._c = c
+        self._last = (-1, c)      # rows of the last call and their struct, never changed once made
 
     def to_c(self, rows: int) -> _lib.dh_token_tables:
-        c = _lib.dh_token_tables()
-        C.pointer(c)[0] = self._c
-        c.rows = rows
+        last, c = self._last
+        if last != rows:
+            c = _lib.dh_token_tables()
+            C.pointer(c)[0] = self._c
+            c.rows = rows
+            self._last = (rows, c)
         return c
 
 
 def _status_ptr(status, device: int):
     if status is None:
         return None
-    if status.dtype != _torch().int32 or status.numel() < 1:
+    if status.dtype is not _torch().int32 or status.numel() < 1:
         raise DhError(_lib.DH_EINVAL, "status must be an int32 tensor")
     _on_device(status, device, "status")
     return status.data_ptr()
@@ -166,6 +194,7 @@ class AttentionConfig:
         self.gqa_mapping = _lib.GQA_TILED         # ReferenceBackend's Tensor::repeat
         self.q_dtype = _lib.DTYPE_BF16
         self.kv_format = _lib.KV_BF16
+        self._last = (None, None)                 # fields of the last _shared_c() and its struct
 
     @classmethod
     def new(cls, num_heads: int, num_kv_heads: int, head_dim: int) -> "AttentionConfig":
@@ -190,6 +219,16 @@ class AttentionConfig:
         c.gqa_mapping = self.gqa_mapping
         c.q_dtype = self.q_dtype
         c.kv_format = self.kv_format
+        return c
+
+    def _shared_c(self) -> _lib.dh_attn_config:
+        """to_c(), made again only when a field has changed; for reading."""
+        key = (self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.sliding_window, self.gqa_mapping,
+               self.q_dtype, self.kv_format)
+        last, c = self._last
+        if last != key:
+            c = self.to_c()
+            self._last = (key, c)
         return c
 
 
@@ -303,14 +342,13 @@ class Pool:
         dev = self.backend.device
         if tables.device != dev:
             raise DhError(_lib.DH_EINVAL, f"tables are on cuda:{tables.device}, the pool on cuda:{dev}")
-        if k.dtype != v.dtype or k.shape != v.shape:
+        if k.dtype is not v.dtype or k.shape != v.shape:
             raise DhError(_lib.DH_EINVAL, f"k is {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
         ks = _rows(k, self.num_kv_heads, self.head_dim, dev, "k")
         vs = _rows(v, self.num_kv_heads, self.head_dim, dev, "v")
-        try:
-            code = dtype_code(k.dtype)
-        except KeyError:
-            raise DhError(_lib.DH_EINVAL, f"row dtype {k.dtype} (float32, bfloat16 or float16)") from None
+        code = _code(k)
+        if code is None:
+            raise DhError(_lib.DH_EINVAL, f"row dtype {k.dtype} (float32, bfloat16 or float16)")
         check(call(self._h, C.byref(tables.to_c(k.shape[0])), k.data_ptr(), v.data_ptr(), ks, vs, code,
                    _status_ptr(status, dev), _device_stream(stream, dev)))
 
@@ -551,7 +589,7 @@ def attend_window(backend: Backend, pool: Pool, config: AttentionConfig, tables:
     dev = backend.device
     if tables.device != dev:
         raise DhError(_lib.DH_EINVAL, f"tables are on cuda:{tables.device}, the backend on cuda:{dev}")
-    if q.dtype != torch_dtype(config.q_dtype) or out.dtype != q.dtype or q.shape != out.shape:
+    if out.dtype is not q.dtype or q.shape != out.shape or _code(q) != config.q_dtype:
         raise DhError(_lib.DH_EINVAL, f"q is {q.dtype} {tuple(q.shape)}, out {out.dtype} {tuple(out.shape)}, the "
                       f"config's {torch_dtype(config.q_dtype)}")
     if sinks < 0:
@@ -562,7 +600,7 @@ def attend_window(backend: Backend, pool: Pool, config: AttentionConfig, tables:
     if workspace is not None:
         _on_device(workspace, dev, "workspace")
         ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    check(lib().dh_attend_window(backend._h, pool._h, C.byref(config.to_c()), min(sinks, 0xFFFFFFFF),
+    check(lib().dh_attend_window(backend._h, pool._h, C.byref(config._shared_c()), min(sinks, 0xFFFFFFFF),
                                  C.byref(tables.to_c(q.shape[0])), q.data_ptr(), qs, out.data_ptr(), os_, ws, nbytes,
                                  _status_ptr(status, dev), _device_stream(stream, dev)))
 
