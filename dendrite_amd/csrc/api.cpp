@@ -1342,6 +1342,7 @@ dh_status token_copy(const dh_pool* p, const dh_token_tables* t, const void* k, 
 // workspace is sized by the same rule.
 struct WindowPlan {
     bool wide, ring;           // query rows in wide blocks; pages straight to LDS
+    uint32_t waves;            // of a narrow workgroup
     uint32_t splits;
     uint32_t window, sinks;
     size_t o_bytes, bytes;     // workspace: O, all
@@ -1397,7 +1398,14 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     const uint64_t pages = w.window ? std::min(all, (w.sinks + 15) / 16 + (w.window + tokens + 14) / 16 + 1) : all;
     const uint64_t blocks = (t.q_indptr ? rows / block + t.batch_size : t.batch_size * ((r + block - 1) / block)) *
                             c.num_kv_heads;
-    const uint64_t cap = !w.wide ? dh::kWaves * (dh::kNarrowWavePages - 2)
+    // Many waves a workgroup where they save a merge: lists too short to be
+    // split (one sequence of 512 tokens, window 256, f32: 10.0 us, and 11.1 with
+    // four waves), or blocks that fill half the chip (64 sequences of 5000 tokens
+    // in FP8, 4 KV heads of 64: 33 us, and 41 with four waves in two parts).
+    // Long lists of few blocks are faster in parts on many CUs (one sequence of
+    // 5000 tokens: 13 us, and 18 with 16 waves).
+    w.waves = blocks <= 256 && (blocks > 128 || pages < 32) ? dh::narrow_waves(c.head_dim) : dh::kWaves;
+    const uint64_t cap = !w.wide ? w.waves * (dh::kNarrowWavePages - 2)
                                  : (w.ring ? dh::kRingMaxPages : dh::kWideMaxPages) - 8;
     const uint64_t least = std::max<uint64_t>(1, (pages + cap - 1) / cap);
     if (w.wide) {
@@ -1405,8 +1413,8 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
         const uint64_t filled = (rows + t.batch_size * block / 2 + block / 2 - 1) / block * c.num_kv_heads;
         w.splits = wide_splits(c, w.ring, uint64_t(t.rows) * c.num_heads, filled, pages, least);
     } else {
-        const uint64_t want = 512u / std::max<uint64_t>(1, blocks);
-        w.splits = uint32_t(std::max(least, std::min(want, pages / 16)));
+        const uint64_t want = 2048 / w.waves / std::max<uint64_t>(1, blocks);
+        w.splits = uint32_t(std::max(least, std::min(want, pages / (4 * w.waves))));
     }
     if (w.splits > 1) {
         const size_t states = size_t(t.rows) * c.num_heads * w.splits;
@@ -1484,7 +1492,7 @@ dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_co
     a.splits = w.splits;
     a.status = status;
     hipError_t e = hipError_t(
-        !w.wide  ? dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, stream)
+        !w.wide  ? dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, w.waves, stream)
         : w.ring ? dh::launch_window_ring(a, c.q_dtype, c.head_dim, stream)
                  : dh::launch_window_wide(a, c.q_dtype, c.kv_format, c.head_dim, stream));
     if (e != hipSuccess) return fail(DH_EHIP, "window attention launch failed: %s", hipGetErrorString(e));

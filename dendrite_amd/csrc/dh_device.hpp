@@ -258,6 +258,9 @@ struct WindowArgs {
 // directly (window_ring.hip) and of one fed through registers; pages a wave of
 // a narrow block and a wide block may be given (registers, LDS lists).
 constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256;
+// Waves of a narrow workgroup where there are few: as many as the registers
+// allow (D = 64: 128, 128: 256 a wave).
+DH_HOST_DEVICE constexpr uint32_t narrow_waves(uint32_t head_dim) { return head_dim == 64 ? 16u : head_dim == 128 ? 8u : 4u; }
 constexpr int kRingShift = 7;
 constexpr uint32_t kRingRows = 1u << kRingShift, kRingMaxPages = 2048, kWideMaxPages = 384;
 // Parts that are merged 16 rows a workgroup; more are merged one row a
@@ -326,7 +329,8 @@ constexpr uint32_t kCsrMinChunk = 1, kCsrMaxChunk = uint32_t(kWaveIdRegs) * 64;
 // Token operators (token_kernels.hip, window_kernels.hip).
 int launch_append_tokens(const TokenCopyArgs& a, uint32_t src_dtype, uint32_t fmt, uint32_t d, void* stream);
 int launch_read_tokens(const TokenCopyArgs& a, uint32_t dst_dtype, uint32_t fmt, uint32_t d, void* stream);
-int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, uint32_t waves,
+                         void* stream);
 int launch_window_wide(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
 int launch_window_ring(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);

@@ -19,27 +19,6 @@ namespace {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Sequence of unit u and u's number in it.  Every lane of the wave calls it.
-__device__ __forceinline__ uint32_t find_sequence(const TokenTables& t, uint64_t u, uint32_t mul,
-                                                  uint32_t shift, uint32_t pad, uint32_t& unit) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = 0, n = t.batch;      // the answer is in [lo, lo + n)
-    uint64_t base = 0;
-    while (true) {
-        const uint32_t step = (n + 63) / 64, b = lo + lane * step;
-        const bool in = lane * step < n;
-        const uint64_t f = in ? (uint64_t(uint32_t(t.q_indptr[b])) * mul >> shift) + uint64_t(pad) * b : ~0ull;
-        const uint64_t m = __ballot(in && f <= u);
-        const int at = m ? 63 - __builtin_clzll(m) : 0;
-        base = __shfl(f, at, 64);
-        lo += at * step;
-        if (step == 1) break;
-        n = min(step, t.batch - lo);
-    }
-    unit = uint32_t(uniform(int(u >= base && u - base < 0xFFFFFFFFull ? uint32_t(u - base) : 0xFFFFFFFFu)));
-    return uint32_t(uniform(int(lo)));
-}
-
 // What sequence b holds.  ok: its entries are in order (dh_token_tables);
 // rows_ok: its rows at least are (row0 .. row0 + nrows inside the call's).
 struct Sequence {
@@ -50,10 +29,9 @@ struct Sequence {
     bool ok, rows_ok;
 };
 
-__device__ __forceinline__ Sequence load_sequence(const TokenTables& t, uint32_t b) {
+// Sequence b from its table entries p0 .. p1, length, and rows r0 .. r1.
+__device__ __forceinline__ Sequence make_sequence(const TokenTables& t, int p0, int p1, int len, int r0, int r1) {
     Sequence s;
-    const int p0 = t.indptr[b], p1 = t.indptr[b + 1], len = t.kv_len[b];
-    const int r0 = t.q_indptr ? t.q_indptr[b] : int(b), r1 = t.q_indptr ? t.q_indptr[b + 1] : int(b) + 1;
     s.page0 = p0;
     s.len = len;
     s.row0 = r0;
@@ -63,6 +41,11 @@ __device__ __forceinline__ Sequence load_sequence(const TokenTables& t, uint32_t
     s.ok = s.rows_ok && p0 >= 0 && p1 >= p0 && uint32_t(p1) <= t.num_indices && len >= 0 &&
            uint32_t(len) <= t.max_kv_len && (int64_t(len) + kPageSize - 1) / kPageSize <= p1 - p0 && s.n <= len;
     return s;
+}
+
+__device__ __forceinline__ Sequence load_sequence(const TokenTables& t, uint32_t b) {
+    const int r0 = t.q_indptr ? t.q_indptr[b] : int(b), r1 = t.q_indptr ? t.q_indptr[b + 1] : int(b) + 1;
+    return make_sequence(t, t.indptr[b], t.indptr[b + 1], t.kv_len[b], r0, r1);
 }
 
 __device__ __forceinline__ Sequence uniform_sequence(const Sequence& x) {
@@ -77,12 +60,44 @@ __device__ __forceinline__ Sequence uniform_sequence(const Sequence& x) {
     return s;
 }
 
-// Reports refused sequences: workgroup w of the launch looks at sequences
-// w * blockDim.x + tid, so a launch of at least batch / blockDim.x workgroups
-// looks at all, whichever units find them.
-__device__ __forceinline__ void report_bad_tables(const TokenTables& t, int32_t* status, uint64_t wg) {
-    const uint64_t b = wg * blockDim.x + threadIdx.x;
-    if (status && b < t.batch && !load_sequence(t, uint32_t(b)).ok) *status = DH_EINVAL;
+// Sequence of unit u and u's number in it.  Every lane of the wave calls it.
+// The last of its levels brings what the sequence holds along: a small call's
+// time is its dependent loads.
+__device__ __forceinline__ Sequence find_sequence(const TokenTables& t, uint64_t u, uint32_t mul, uint32_t shift,
+                                                  uint32_t pad, uint32_t& unit) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0, n = t.batch;      // the answer is in [lo, lo + n)
+    auto number = [&](uint32_t b, int q) { return (uint64_t(uint32_t(q)) * mul >> shift) + uint64_t(pad) * b; };
+    while (n > 64) {
+        const uint32_t step = (n + 63) / 64, b = min(lo + lane * step, t.batch - 1);
+        const uint64_t m = __ballot(lane * step < n && number(b, t.q_indptr[b]) <= u);
+        lo += uint32_t(m ? 63 - __builtin_clzll(m) : 0) * step;
+        n = min(step, t.batch - lo);
+    }
+    const uint32_t b = min(lo + lane, t.batch - 1);
+    const int r0 = t.q_indptr[b], r1 = t.q_indptr[b + 1], p0 = t.indptr[b], p1 = t.indptr[b + 1], len = t.kv_len[b];
+    const uint64_t m = __ballot(lane < n && number(b, r0) <= u);
+    const int at = uniform(m ? 63 - __builtin_clzll(m) : 0);
+    auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+    const Sequence s = make_sequence(t, pick(p0), pick(p1), pick(len), pick(r0), pick(r1));
+    const uint64_t base = number(uint32_t(uniform(int(lo))) + at, pick(r0));
+    unit = uint32_t(uniform(int(u >= base && u - base < 0xFFFFFFFFull ? uint32_t(u - base) : 0xFFFFFFFFu)));
+    return uniform_sequence(s);
+}
+
+// Whether a sequence that falls to this thread is refused: workgroup w of the
+// launch looks at sequences w * blockDim.x + tid (its last ones at the batch's
+// last), so a launch of at least batch / blockDim.x workgroups looks at all,
+// whichever units find them.  A value, to be reported once other loads are
+// under way.
+__device__ __forceinline__ bool sees_refused(const TokenTables& t, uint32_t wg) {
+    const uint64_t first = uint64_t(wg) * blockDim.x;
+    if (first >= t.batch) return false;
+    return !load_sequence(t, uint32_t(min(first + threadIdx.x, uint64_t(t.batch - 1)))).ok;
+}
+
+__device__ __forceinline__ void report(bool refused, int32_t* status) {
+    if (refused && status) *status = DH_EINVAL;
 }
 
 // A table entry as a page of the pool: -1 where it is outside it.

@@ -138,14 +138,14 @@ __device__ __forceinline__ Block find_block(const TokenCopyArgs& a) {
     const uint32_t unit = item / per, ph = item - unit * per;
     k.plane = ph >= a.hkv ? 1u : 0u;
     k.head = ph - k.plane * a.hkv;
-    uint32_t b, u = 0;
+    uint32_t u = 0;
+    Sequence s;
     if (a.t.q_indptr) {
-        b = find_sequence(a.t, unit, 1, 4, 2, u);
+        s = find_sequence(a.t, unit, 1, 4, 2, u);
     } else {
         if (unit >= a.t.batch) return k;
-        b = unit;
+        s = uniform_sequence(load_sequence(a.t, unit));
     }
-    const Sequence s = uniform_sequence(load_sequence(a.t, b));
     if (!s.ok || s.n == 0) return k;
     const int first = s.len - s.n, last_page = (s.len - 1) >> 4;
     if (u > uint32_t(last_page - (first >> 4))) return k;
@@ -162,8 +162,9 @@ template <int D, uint32_t SRC, uint32_t FMT>
 __global__ __launch_bounds__(256) void append_tokens_kernel(TokenCopyArgs a) {
     constexpr int LPR = D / 8, RPI = 64 / LPR, NI = kPageSize / RPI;   // lanes a row, rows a step, steps
     constexpr uint32_t EB = SRC == kF32 ? 4 : 2;
-    report_bad_tables(a.t, a.status, blockIdx.x);
+    const bool refused = sees_refused(a.t, blockIdx.x);
     const Block k = find_block(a);
+    report(refused, a.status);
     if (!k.any) return;
     const int lane = threadIdx.x & 63, cd = lane % LPR, lr = lane / LPR;
     const int id = uniform(a.t.indices[k.entry]);
@@ -261,8 +262,9 @@ __global__ __launch_bounds__(256) void read_tokens_kernel(TokenCopyArgs a) {
     constexpr uint32_t EB = DST == kF32 ? 4 : 2;
     constexpr bool CODES = FMT == kFP8 || FMT == kMX;
     constexpr int SB = CODES ? 1 : (FMT == kF32 ? 4 : 2);
-    report_bad_tables(a.t, a.status, blockIdx.x);
+    const bool refused = sees_refused(a.t, blockIdx.x);
     const Block k = find_block(a);
+    report(refused, a.status);
     if (!k.any) return;
     const int lane = threadIdx.x & 63, cd = lane % LPR, lr = lane / LPR;
     const int page = checked_page(uniform(a.t.indices[k.entry]), a.num_pages, a.status);

@@ -29,16 +29,16 @@ template <int SHIFT>
 __device__ __forceinline__ RowBlock find_rows(const WindowArgs& a, uint64_t unit, int kv_head) {
     RowBlock k{};
     k.kv_head = kv_head;
-    uint32_t b, u;
+    uint32_t u;
     if (a.t.q_indptr) {
-        b = find_sequence(a.t, unit, a.r, SHIFT, 1, u);
+        k.seq = find_sequence(a.t, unit, a.r, SHIFT, 1, u);
     } else {
         const uint32_t per = (a.r + (1u << SHIFT) - 1) >> SHIFT;
         if (unit >= uint64_t(a.t.batch) * per) return k;
-        b = uint32_t(unit) / per;
+        const uint32_t b = uint32_t(unit) / per;
         u = uint32_t(unit) - b * per;
+        k.seq = uniform_sequence(load_sequence(a.t, b));
     }
-    k.seq = uniform_sequence(load_sequence(a.t, b));
     const int64_t rows = int64_t(k.seq.nrows) * a.r, rho0 = int64_t(u) << SHIFT;
     if (rho0 >= rows) return k;
     k.rho0 = int(rho0);

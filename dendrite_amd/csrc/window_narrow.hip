@@ -60,17 +60,17 @@ __device__ __forceinline__ bool all_see(const WindowArgs& a, int pmin, int pmax,
     return t0 + 15 <= pmin && (t0 >= window_lo(a, pmax) || t0 + 15 < a.sinks);
 }
 
-// Joins the states of the workgroup's four waves and writes the block's rows:
+// Joins the states of the workgroup's waves and writes the block's rows:
 // to out, or as one part's state to the workspace.  Lane (g, c) holds
 // O[row c][(4g + i) * EPL + e] = O[e][i], L its row's sum (already over the
 // four lanes of the row) and m the row's reference.
-template <int D, uint32_t QT>
+template <int D, uint32_t QT, int NW>
 __device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& k, int split, float m, float L,
                                            const f4 (&O)[D / 16], float* lds) {
     constexpr int EPL = D / 16, RS = D + 4;          // padded row
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
     float* o = lds + wave * 16 * RS;
-    float* ml = lds + kWaves * 16 * RS;              // [wave][16][2]
+    float* ml = lds + NW * 16 * RS;              // [wave][16][2]
     #pragma unroll
     for (int i = 0; i < 4; ++i)
         #pragma unroll
@@ -82,15 +82,15 @@ __device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& 
     }
     __syncthreads();
     const int row = tid >> 4, d0 = (tid & 15) * EPL;
-    if (row >= k.nrows) return;
+    if (tid >= 256 || row >= k.nrows) return;
     float mx = kNegInf;
     #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[(w * 16 + row) * 2]);
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ml[(w * 16 + row) * 2]);
     float x[EPL], sum = 0.f;
     #pragma unroll
     for (int e = 0; e < EPL; ++e) x[e] = 0.f;
     #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
         const float mw = ml[(w * 16 + row) * 2];
         const float al = mw == kNegInf ? 0.f : fast_exp2(mw - mx);
         sum += al * ml[(w * 16 + row) * 2 + 1];
@@ -130,20 +130,22 @@ __device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& 
 // then parts, then blocks.
 template <int SHIFT>
 __device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& split) {
-    report_bad_tables(a.t, a.status, blockIdx.x);
+    const bool refused = sees_refused(a.t, blockIdx.x);
     const uint32_t x = blockIdx.x / a.hkv;
     const int head = uniform(int(blockIdx.x - x * a.hkv));
     const uint32_t unit = x / a.splits;
     split = uniform(int(x - unit * a.splits));
-    return uniform_block(find_rows<SHIFT>(a, unit, head));
+    const RowBlock k = uniform_block(find_rows<SHIFT>(a, unit, head));
+    report(refused, a.status);
+    return k;
 }
 
-template <int D, uint32_t KVF, bool F16>
-__global__ __launch_bounds__(256) void window_narrow_kernel(WindowArgs a) {
+template <int D, uint32_t KVF, bool F16, int NW>
+__global__ __launch_bounds__(64 * NW) void window_narrow_kernel(WindowArgs a) {
     using R = PageRaw<D, KVF>;
     constexpr int KB = D / 32, EPL = D / 16;
     constexpr uint32_t QT = F16 ? DH_DTYPE_F16 : DH_DTYPE_BF16;
-    __shared__ __attribute__((aligned(16))) float lds[kWaves * 16 * (D + 4) + kWaves * 32];
+    __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (D + 4) + NW * 32];
     int split;
     const RowBlock k = workgroup_rows<4>(a, split);
     if (k.nrows == 0) return;
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(256) void window_narrow_kernel(WindowArgs a) {
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     WavePages pages;
-    pages.load(a, k, split * kWaves + wave, int(a.splits) * kWaves);
+    pages.load(a, k, split * NW + wave, int(a.splits) * NW);
 
     // Query rows as B operands: lane (g, c) holds row c.
     const int rho = k.rho0 + min(c, k.nrows - 1);
@@ -312,14 +314,14 @@ __global__ __launch_bounds__(256) void window_narrow_kernel(WindowArgs a) {
             if (refill) load_v(pi + 1);
         }
     }
-    join_waves<D, QT>(a, k, split, m, L[0], O, lds);
+    join_waves<D, QT, NW>(a, k, split, m, L[0], O, lds);
 }
 
 // f32 queries and cache: one page a step on v_mfma_f32_16x16x4_f32.
-template <int D>
-__global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) {
     constexpr int KQ = D / 4, EPL = D / 16;
-    __shared__ __attribute__((aligned(16))) float lds[kWaves * 16 * (D + 4) + kWaves * 32];
+    __shared__ __attribute__((aligned(16))) float lds[NW * 16 * (D + 4) + NW * 32];
     int split;
     const RowBlock k = workgroup_rows<4>(a, split);
     if (k.nrows == 0) return;
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     WavePages pages;
-    pages.load(a, k, split * kWaves + wave, int(a.splits) * kWaves);
+    pages.load(a, k, split * NW + wave, int(a.splits) * NW);
     const int rho = k.rho0 + min(c, k.nrows - 1);
     int token, head;
     row_place(a, k, rho, token, head);
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(256) void window_narrow32_kernel(WindowArgs a) {
         }
         if (j + 1 < pages.n) load(j + 1);
     }
-    join_waves<D, DH_DTYPE_F32>(a, k, split, m, rowgroup_sum(l), O, lds);
+    join_waves<D, DH_DTYPE_F32, NW>(a, k, split, m, rowgroup_sum(l), O, lds);
 }
 
 // Writes elements 4 col .. 4 col + 3 of a merged row.
@@ -487,26 +489,34 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
     write_merged<D, QT>(a, at, head, col, x, sum);
 }
 
-template <int D>
-hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, dim3 grid, hipStream_t s) {
-    const dim3 block(256);
+template <int D, int NW>
+hipError_t launch_narrow_w(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, dim3 grid, hipStream_t s) {
+    const dim3 block(64 * NW);
     if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32)
-        hipLaunchKernelGGL((window_narrow32_kernel<D>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow32_kernel<D, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_BF16)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_F16)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_FP8)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, false, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_FP8)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, true>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, true, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_MX)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, false, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_MX)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, true>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, true, NW>), grid, block, 0, s, a);
     else
         return hipErrorInvalidValue;
     return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t waves, dim3 grid, hipStream_t s) {
+    if constexpr (narrow_waves(D) != kWaves) {
+        if (waves == narrow_waves(D)) return launch_narrow_w<D, int(narrow_waves(D))>(a, q_dtype, fmt, grid, s);
+    }
+    return waves == kWaves ? launch_narrow_w<D, kWaves>(a, q_dtype, fmt, grid, s) : hipErrorInvalidValue;
 }
 
 template <int D, uint32_t QT>
@@ -529,15 +539,16 @@ hipError_t launch_merge_w(const WindowArgs& a, uint32_t q_dtype, uint32_t blocks
 
 }  // namespace
 
-int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream) {
+int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, uint32_t waves,
+                         void* stream) {
     const uint64_t blocks = row_blocks(a, 4) * a.splits * a.hkv;
     if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
     const dim3 grid{uint32_t(blocks)};
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (d) {
-        case 64: return launch_narrow_d<64>(a, q_dtype, fmt, grid, s);
-        case 128: return launch_narrow_d<128>(a, q_dtype, fmt, grid, s);
-        case 256: return launch_narrow_d<256>(a, q_dtype, fmt, grid, s);
+        case 64: return launch_narrow_d<64>(a, q_dtype, fmt, waves, grid, s);
+        case 128: return launch_narrow_d<128>(a, q_dtype, fmt, waves, grid, s);
+        case 256: return launch_narrow_d<256>(a, q_dtype, fmt, waves, grid, s);
         default: return hipErrorInvalidValue;
     }
 }

@@ -119,11 +119,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
     static_assert(kRingRows == RT * kWaves * kTileRows, "rows a block");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[C::RING];
     __shared__ int ids[kRingMaxPages + 2 * (P + 1)];
-    report_bad_tables(a.t, a.status, blockIdx.x);
+    const bool refused = sees_refused(a.t, blockIdx.x);
     const uint32_t x0 = blockIdx.x / a.hkv;
     const uint32_t unit = x0 / a.splits;
     const int split = uniform(int(x0 - unit * a.splits));
     const RowBlock k = uniform_block(find_rows<kRingShift>(a, unit, int(blockIdx.x - x0 * a.hkv)));
+    report(refused, a.status);
     if (k.nrows == 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     if (k.zero) {

@@ -334,11 +334,12 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
     __shared__ __attribute__((aligned(1024))) uint8_t tiles[C::RING * C::TILE];
     __shared__ int ids[kWideMaxPages + (C::RING + C::AHEAD + 2) * NP];        // (read ahead)
     __shared__ __attribute__((aligned(16))) f2 scl[KVF == KVF_FP8 ? kWideMaxPages + 2 * NP : 1];
-    report_bad_tables(a.t, a.status, blockIdx.x);
+    const bool refused = sees_refused(a.t, blockIdx.x);
     const uint32_t x0 = blockIdx.x / a.hkv;
     const uint32_t unit = x0 / a.splits;
     const int split = uniform(int(x0 - unit * a.splits));
     const RowBlock k = uniform_block(find_rows<C::SHIFT>(a, unit, int(blockIdx.x - x0 * a.hkv)));
+    report(refused, a.status);
     if (k.nrows == 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, c = lane & 31;
     if (k.zero) {
