@@ -1399,12 +1399,16 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     const uint64_t blocks = (t.q_indptr ? rows / block + t.batch_size : t.batch_size * ((r + block - 1) / block)) *
                             c.num_kv_heads;
     // Many waves a workgroup where they save a merge: lists too short to be
-    // split (one sequence of 512 tokens, window 256, f32: 10.0 us, and 11.1 with
+    // split (one sequence of 512 tokens, window 256, f32: 9.7 us, and 11.1 with
     // four waves), or blocks that fill half the chip (64 sequences of 5000 tokens
-    // in FP8, 4 KV heads of 64: 33 us, and 41 with four waves in two parts).
+    // in FP8, 4 KV heads of 64: 32 us, and 41 with four waves in two parts), in
+    // 8-bit caches all of it (70 sequences: 46 us, and 65; but 90 and 79 in bf16).
     // Long lists of few blocks are faster in parts on many CUs (one sequence of
     // 5000 tokens: 13 us, and 18 with 16 waves).
-    w.waves = blocks <= 256 && (blocks > 128 || pages < 32) ? dh::narrow_waves(c.head_dim) : dh::kWaves;
+    w.waves = dh::kWaves;
+    while (2 * w.waves <= dh::narrow_waves(c.head_dim) && 2 * w.waves * blocks <= 256 * dh::narrow_waves(c.head_dim) &&
+           (blocks > 128 || pages < 32) && (blocks <= 256 || codes))
+        w.waves *= 2;
     const uint64_t cap = !w.wide ? w.waves * (dh::kNarrowWavePages - 2)
                                  : (w.ring ? dh::kRingMaxPages : dh::kWideMaxPages) - 8;
     const uint64_t least = std::max<uint64_t>(1, (pages + cap - 1) / cap);

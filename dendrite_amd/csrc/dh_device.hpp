@@ -258,8 +258,8 @@ struct WindowArgs {
 // directly (window_ring.hip) and of one fed through registers; pages a wave of
 // a narrow block and a wide block may be given (registers, LDS lists).
 constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256;
-// Waves of a narrow workgroup where there are few: as many as the registers
-// allow (D = 64: 128, 128: 256 a wave).
+// Most waves of a narrow workgroup, as the registers allow (D = 64: 128 a wave,
+// D = 128: 256).
 DH_HOST_DEVICE constexpr uint32_t narrow_waves(uint32_t head_dim) { return head_dim == 64 ? 16u : head_dim == 128 ? 8u : 4u; }
 constexpr int kRingShift = 7;
 constexpr uint32_t kRingRows = 1u << kRingShift, kRingMaxPages = 2048, kWideMaxPages = 384;

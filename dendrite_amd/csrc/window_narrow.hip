@@ -140,8 +140,17 @@ __device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& spl
     return k;
 }
 
+// Waves a SIMD the registers are to leave room for.  8-bit pages are converted a
+// block of dims at a time, as the products take them, and need few: whole
+// operands (64 sequences of 5000 tokens in MXFP8, 64 heads of 128: 129 us
+// against 126, 40 of 2000: 45 against 39; 32 verifying 6 tokens, 16 heads of
+// 256, window 2001: 61 against 49) leave room for one wave less, at 256 dims for
+// one only.
+template <int D, bool CODES>
+constexpr int kNarrowPerSimd = !CODES ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4;
+
 template <int D, uint32_t KVF, bool F16, int NW>
-__global__ __launch_bounds__(64 * NW) void window_narrow_kernel(WindowArgs a) {
+__global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>)) void window_narrow_kernel(WindowArgs a) {
     using R = PageRaw<D, KVF>;
     constexpr int KB = D / 32, EPL = D / 16;
     constexpr uint32_t QT = F16 ? DH_DTYPE_F16 : DH_DTYPE_BF16;
@@ -216,12 +225,11 @@ __global__ __launch_bounds__(64 * NW) void window_narrow_kernel(WindowArgs a) {
     }
     #pragma unroll 1
     for (int pi = 0; pi < npairs; ++pi) {
-        // 8-bit pages are loaded again as soon as they are converted, past the
-        // list's end too (page 0): a load on some paths only makes every wait
-        // for others stricter (64 sequences of 5000 tokens in MXFP8, 64 heads of
-        // 128: 132 us, and 144 with 16 bits' order).  16-bit pages lose more by
-        // those extra loads (32 sequences of 3 new tokens, 32 heads of 64, window
-        // 2001: 32 us, and 30 in theirs).
+        // 8-bit pages are loaded past the list's end too (page 0): a load on some
+        // paths only makes every wait for others stricter (64 sequences of 5000
+        // tokens in MXFP8, 64 heads of 128: 132 us, and 144 with the branch).
+        // 16-bit pages lose more by those extra loads (32 sequences of 3 new
+        // tokens, 32 heads of 64, window 2001: 32 us, and 30 with the branch).
         const bool refill = R::FP8 || pi + 1 < npairs;
         int t0[2];
         bool ok[2], full = true;
@@ -231,33 +239,43 @@ __global__ __launch_bounds__(64 * NW) void window_narrow_kernel(WindowArgs a) {
             t0[q] = 16 * list_page(k, pages.j0 + 2 * pi + q);
             full = full && ok[q] && all_see(a, k.pmin, k.pmax, t0[q]);
         }
-        uint32_t kop[2][KB][4];
         f4 s[1][2];
-        k_operand<D, KVF, F16>(pr[0], kop[0]);
-        k_operand<D, KVF, F16>(pr[1], kop[1]);
-        pair_scores<D, F16, 1, 1>(kop[0], kop[1], qB, s);
+        if constexpr (R::FP8) {
+            s[0][0] = s[0][1] = f4{0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                #pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const float sc = KVF == KVF_MX ? e8m0_to_float(pr[q].ksc[kb]) : 1.f;
+                    uint32_t op[4];
+                    e4m3x4_cvt<F16>(pr[q].k[kb][0], sc, op[0], op[1]);
+                    e4m3x4_cvt<F16>(pr[q].k[kb][1], sc, op[2], op[3]);
+                    s[0][q] = mma16<F16>(op, qB[0][kb], s[0][q]);
+                }
+        } else {
+            uint32_t kop[2][KB][4];
+            k_operand<D, KVF, F16>(pr[0], kop[0]);
+            k_operand<D, KVF, F16>(pr[1], kop[1]);
+            pair_scores<D, F16, 1, 1>(kop[0], kop[1], qB, s);
+        }
         // A scale of zero (a page nobody wrote) must not meet a masked -inf.
         const float f0 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[0], 1e-30f) : a.scale_log2;
         const float f1 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[1], 1e-30f) : a.scale_log2;
         const float v0s = vs[0], v1s = vs[1];
         if (refill) load_k(pi + 1);
-        uint32_t vop[2][4][D / 32];
-        #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        // V of tokens nobody sees: their weights are zero, but what lies there
+        // need not be a number.
+        if (!full) {
             #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool keep = full || (ok[q] && any.sees(t0[q] + 4 * g + j));
-                if constexpr (!R::FP8) {
+            for (int q = 0; q < 2; ++q)
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool keep = ok[q] && any.sees(t0[q] + 4 * g + j);
                     #pragma unroll
-                    for (int w = 0; w < R::VW; ++w) vop[q][j][w] = keep ? pr[q].v[j][w] : 0u;
-                } else {
-                    const float sc = KVF == KVF_MX && keep ? e8m0_to_float(pr[q].vsc[j]) : 1.f;
-                    #pragma unroll
-                    for (int w = 0; w < R::VW; ++w)
-                        e4m3x4_cvt<F16>(keep ? pr[q].v[j][w] : 0u, sc, vop[q][j][2 * w], vop[q][j][2 * w + 1]);
+                    for (int w = 0; w < R::VW; ++w) pr[q].v[j][w] = keep ? pr[q].v[j][w] : 0u;
+                    if constexpr (KVF == KVF_MX) pr[q].vsc[j] = keep ? pr[q].vsc[j] : 127u;
                 }
-            }
-        if constexpr (R::FP8) load_v(pi + 1);
+        }
         float x[8];
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -300,19 +318,33 @@ __global__ __launch_bounds__(64 * NW) void window_narrow_kernel(WindowArgs a) {
             pk[2] = pack2(x[4] * v1s, x[5] * v1s, F16);
             pk[3] = pack2(x[6] * v1s, x[7] * v1s, F16);
         }
-        #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int w = e >> 1;
+        // O^T += V^T P^T of dims e, given its dword w of tokens (q, j)
+        auto product = [&](int e, auto&& w) __attribute__((always_inline)) {
             const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
-            const uint32_t vA[4] = {__builtin_amdgcn_perm(vop[0][1][w], vop[0][0][w], sel),
-                                    __builtin_amdgcn_perm(vop[0][3][w], vop[0][2][w], sel),
-                                    __builtin_amdgcn_perm(vop[1][1][w], vop[1][0][w], sel),
-                                    __builtin_amdgcn_perm(vop[1][3][w], vop[1][2][w], sel)};
+            const uint32_t vA[4] = {__builtin_amdgcn_perm(w(0, 1), w(0, 0), sel), __builtin_amdgcn_perm(w(0, 3), w(0, 2), sel),
+                                    __builtin_amdgcn_perm(w(1, 1), w(1, 0), sel), __builtin_amdgcn_perm(w(1, 3), w(1, 2), sel)};
             O[e] = mma16<F16>(vA, pk, O[e]);
+        };
+        if constexpr (R::FP8) {
+            #pragma unroll
+            for (int i = 0; i < R::VW; ++i) {      // four dims
+                uint32_t op[2][4][2];
+                #pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        e4m3x4_cvt<F16>(pr[q].v[j][i], KVF == KVF_MX ? e8m0_to_float(pr[q].vsc[j]) : 1.f, op[q][j][0],
+                                        op[q][j][1]);
+                #pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    product(4 * i + e, [&](int q, int j) __attribute__((always_inline)) { return op[q][j][e >> 1]; });
+            }
+        } else {
+            #pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                product(e, [&](int q, int j) __attribute__((always_inline)) { return pr[q].v[j][e >> 1]; });
         }
-        if constexpr (!R::FP8) {
-            if (refill) load_v(pi + 1);
-        }
+        if (refill) load_v(pi + 1);
     }
     join_waves<D, QT, NW>(a, k, split, m, L[0], O, lds);
 }
@@ -513,8 +545,11 @@ hipError_t launch_narrow_w(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, 
 
 template <int D>
 hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t waves, dim3 grid, hipStream_t s) {
-    if constexpr (narrow_waves(D) != kWaves) {
-        if (waves == narrow_waves(D)) return launch_narrow_w<D, int(narrow_waves(D))>(a, q_dtype, fmt, grid, s);
+    if constexpr (narrow_waves(D) >= 16) {
+        if (waves == 16) return launch_narrow_w<D, 16>(a, q_dtype, fmt, grid, s);
+    }
+    if constexpr (narrow_waves(D) >= 8) {
+        if (waves == 8) return launch_narrow_w<D, 8>(a, q_dtype, fmt, grid, s);
     }
     return waves == kWaves ? launch_narrow_w<D, kWaves>(a, q_dtype, fmt, grid, s) : hipErrorInvalidValue;
 }
