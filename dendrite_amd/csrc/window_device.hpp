@@ -85,6 +85,16 @@ __device__ __forceinline__ void row_place(const WindowArgs& a, const RowBlock& k
     head = a.tiled ? k.kv_head + j * int(a.hkv) : k.kv_head * int(a.r) + j;
 }
 
+// FP8 blocks: V's scale v goes into the weights, as log2 v beside the score, so
+// that the reference a row's weights are kept near is that of weight times
+// scale: 16-bit weights then keep their precision whatever the scale.  Below
+// 2^-64, the least that an append writes, a scale counts as that (a page nobody
+// wrote may hold zero).  The row's sum takes the scales out again, 2^(s - m) up
+// to 2^(64 + 8) a token and down to 2^-119 for the largest scales: it is counted
+// in units of 2^-32, which keeps either end within f32.
+constexpr float kSumUnitLog2 = 32.f, kSumUnit = 0x1p-32f;
+__device__ __forceinline__ float value_log2(float v) { return __builtin_amdgcn_logf(fmaxf(v, 0x1p-64f)); }
+
 // Zero rows of a refused or unused sequence.
 typedef uint32_t word16 __attribute__((ext_vector_type(4)));
 template <int D, uint32_t QT>

@@ -187,8 +187,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
     row.sinks = a.sinks;
     const Sight any{k.pmax, window_lo(a, k.pmin), a.sinks};    // what some row of the block sees
 
-    float m = kNegInf;
-    f4 L = {0.f, 0.f, 0.f, 0.f};
+    float m = kNegInf, l = 0.f;
     f4 O[EPL];
     #pragma unroll
     for (int e = 0; e < EPL; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
         // A scale of zero (a page nobody wrote) must not meet a masked -inf.
         const float f0 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[0], 1e-30f) : a.scale_log2;
         const float f1 = KVF == KVF_FP8 ? fmaxf(a.scale_log2 * ks[1], 1e-30f) : a.scale_log2;
-        const float v0s = vs[0], v1s = vs[1];
+        const float v0 = KVF == KVF_FP8 ? value_log2(vs[0]) : 0.f, v1 = KVF == KVF_FP8 ? value_log2(vs[1]) : 0.f;
         if (refill) load_k(pi + 1);
         // V of tokens nobody sees: their weights are zero, but what lies there
         // need not be a number.
@@ -290,7 +289,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
             }
         }
         const float r0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), r1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
-        const float lm = fmaxf(r0 * f0, r1 * f1);
+        const float lm = KVF == KVF_FP8 ? fmaxf(__builtin_fmaf(r0, f0, v0), __builtin_fmaf(r1, f1, v1)) : fmaxf(r0 * f0, r1 * f1);
         // The reference moves only when a score passes it by 8 (2^8 at most
         // then), so the accumulators are seldom rescaled.
         if (__ballot(lm > m + 8.f)) {
@@ -298,32 +297,39 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
             const float mnew = mx > m + 8.f ? mx : m;
             const float alpha = m == kNegInf ? 0.f : fast_exp2(m - mnew);
             m = mnew;
-            L *= alpha;
+            l *= alpha;
             #pragma unroll
             for (int e = 0; e < EPL; ++e) O[e] *= alpha;
         }
         const float nm = m == kNegInf ? 0.f : -m;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = fast_exp2(__builtin_fmaf(x[i], f0, nm));
-            x[4 + i] = fast_exp2(__builtin_fmaf(x[4 + i], f1, nm));
+            x[i] = fast_exp2(__builtin_fmaf(x[i], f0, nm + v0));
+            x[4 + i] = fast_exp2(__builtin_fmaf(x[4 + i], f1, nm + v1));
         }
-        const uint32_t one2 = F16 ? 0x3C003C00u : 0x3F803F80u;
-        const uint32_t ones[4] = {one2, one2, one2, one2};
-        uint32_t pk[4] = {pack2(x[0], x[1], F16), pack2(x[2], x[3], F16), pack2(x[4], x[5], F16), pack2(x[6], x[7], F16)};
-        L = mma16<F16>(ones, pk, L);        // the sum of the weights as V gets them
-        if constexpr (KVF == KVF_FP8) {
-            pk[0] = pack2(x[0] * v0s, x[1] * v0s, F16);
-            pk[1] = pack2(x[2] * v0s, x[3] * v0s, F16);
-            pk[2] = pack2(x[4] * v1s, x[5] * v1s, F16);
-            pk[3] = pack2(x[6] * v1s, x[7] * v1s, F16);
+        // Each weight as two 16-bit numbers, the second the first one's rounding
+        // error: alone, the first's errors (2^-9 relative in bf16, 2^-12 in f16)
+        // are in the output as large as its own rounding, whatever the number of
+        // tokens.  The sum is of the weights before that, in f32.  A wave waits
+        // for its pages: the second products cost it 1 %.
+        uint32_t hi[4], lo[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = pack2(x[2 * i], x[2 * i + 1], F16);
+            lo[i] = pack2(x[2 * i] - unpack_lo(hi[i], F16), x[2 * i + 1] - unpack_hi(hi[i], F16), F16);
         }
+        const float l0 = (x[0] + x[1]) + (x[2] + x[3]), l1 = (x[4] + x[5]) + (x[6] + x[7]);
+        if constexpr (KVF == KVF_FP8)
+            l = __builtin_fmaf(l0, fast_exp2(kSumUnitLog2 - v0), __builtin_fmaf(l1, fast_exp2(kSumUnitLog2 - v1), l));
+        else
+            l += l0 + l1;
         // O^T += V^T P^T of dims e, given its dword w of tokens (q, j)
         auto product = [&](int e, auto&& w) __attribute__((always_inline)) {
             const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
             const uint32_t vA[4] = {__builtin_amdgcn_perm(w(0, 1), w(0, 0), sel), __builtin_amdgcn_perm(w(0, 3), w(0, 2), sel),
                                     __builtin_amdgcn_perm(w(1, 1), w(1, 0), sel), __builtin_amdgcn_perm(w(1, 3), w(1, 2), sel)};
-            O[e] = mma16<F16>(vA, pk, O[e]);
+            O[e] = mma16<F16>(vA, hi, O[e]);
+            O[e] = mma16<F16>(vA, lo, O[e]);
         };
         if constexpr (R::FP8) {
             #pragma unroll
@@ -346,7 +352,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
         }
         if (refill) load_v(pi + 1);
     }
-    join_waves<D, QT, NW>(a, k, split, m, L[0], O, lds);
+    join_waves<D, QT, NW>(a, k, split, m, rowgroup_sum(l) * (KVF == KVF_FP8 ? kSumUnit : 1.f), O, lds);
 }
 
 // f32 queries and cache: one page a step on v_mfma_f32_16x16x4_f32.

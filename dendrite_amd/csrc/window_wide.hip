@@ -208,15 +208,18 @@ __device__ __forceinline__ void wide_v(const WideReads<D>& r, uint32_t at, u32x4
         }
 }
 
-// Largest scaled score of the lane's 16 (page factors f).
-__device__ __forceinline__ float wide_max(const f16v& s, float f0, float f1) {
+// Largest scaled score of the lane's 16, as the reference counts it (the pages'
+// factors and log2 V scales fac).
+template <uint32_t KVF>
+__device__ __forceinline__ float wide_max(const f16v& s, const f4& fac) {
     float a = s[0], b = s[8];
     #pragma unroll
     for (int i = 1; i < 8; ++i) {
         a = fmaxf(a, s[i]);
         b = fmaxf(b, s[8 + i]);
     }
-    return fmaxf(a * f0, b * f1);
+    if constexpr (KVF == KVF_FP8) return fmaxf(__builtin_fmaf(a, fac[0], fac[1]), __builtin_fmaf(b, fac[2], fac[3]));
+    return fmaxf(a * fac[0], b * fac[2]);
 }
 
 // O *= alpha.  With one wave a SIMD, O lives in the accumulation half of the
@@ -271,29 +274,25 @@ __device__ __forceinline__ float add2(uint32_t w, float c) {
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, w), s16x2{0x3F80, 0x3F80}, c, false);
 }
 
-// Weights of 32 tokens as the B operand, V's block scales v0 / v1 on them.  The
-// row's sum is of the weights as V gets them, but for the block scales.
+// Weights of 32 tokens as the B operand: 2^(s - m), with V's block scale in the
+// exponent.  The row's sum is of the weights as V gets them, in kSumUnit where
+// the scales are taken out of it again.
 template <uint32_t KVF, bool F16>
-__device__ __forceinline__ void wide_weights(const f16v& s, float f0, float f1, float v0, float v1, float m, float& L,
-                                             u32x4 (&pk)[2]) {
+__device__ __forceinline__ void wide_weights(const f16v& s, const f4& fac, float m, float& L, u32x4 (&pk)[2]) {
     const float nm = m == kNegInf ? 0.f : -m;
     #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        float x[8];
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = fast_exp2(__builtin_fmaf(s[8 * g + i], g ? f1 : f0, nm));
-            if constexpr (KVF == KVF_FP8) {
-                L += x[i];
-                x[i] *= g ? v1 : v0;
-            }
-        }
         uint32_t w[4];
+        float l = KVF == KVF_FP8 ? 0.f : L;
+        const float c = KVF == KVF_FP8 ? nm + fac[2 * g + 1] : nm;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = pack2(x[2 * i], x[2 * i + 1], F16);
-            if constexpr (KVF != KVF_FP8) L = add2<F16>(w[i], L);
+            const float x0 = fast_exp2(__builtin_fmaf(s[8 * g + 2 * i], fac[2 * g], c));
+            const float x1 = fast_exp2(__builtin_fmaf(s[8 * g + 2 * i + 1], fac[2 * g], c));
+            w[i] = pack2(x0, x1, F16);
+            l = add2<F16>(w[i], l);
         }
+        L = KVF == KVF_FP8 ? __builtin_fmaf(l, fast_exp2(kSumUnitLog2 - fac[2 * g + 1]), L) : l;
         pk[g] = u32x4{w[0], w[1], w[2], w[3]};
     }
 }
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
                     s = f2{p[0], p[a.hkv]};
                 }
                 // a scale of zero (a page nobody wrote) must not meet a masked -inf
-                scl[j] = f2{fmaxf(a.scale_log2 * s[0], 1e-30f), s[1]};
+                scl[j] = f2{fmaxf(a.scale_log2 * s[0], 1e-30f), value_log2(s[1])};
             }
         }
     }
@@ -433,7 +432,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) s[rt] = wide_scores<D, F16>(kw, q[rt]);
     wide_k<D>(rd, C::TILE, kw);
-    f4 fac = {a.scale_log2, 1.f, a.scale_log2, 1.f};    // the two pages' score factors and V scales
+    f4 fac = {a.scale_log2, 0.f, a.scale_log2, 0.f};    // the two pages' score factors and log2 of V's scales
     if constexpr (KVF == KVF_FP8) fac = *reinterpret_cast<const f4*>(scl);
     uint32_t cur = 0;                           // byte offset of the tile in the ring
     auto step = [&](auto T, int tile) __attribute__((always_inline)) {
@@ -445,7 +444,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
         bool up = false;
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            lm[rt] = wide_max(s[rt], fac[0], fac[2]);
+            lm[rt] = wide_max<KVF>(s[rt], fac);
             up = up || lm[rt] > w[rt].m + 8.f;
         }
         if (__builtin_expect(__ballot(up) != 0, 0)) {
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
         #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             sn[rt] = wide_scores<D, F16>(kw, q[rt]);
-            wide_weights<KVF, F16>(s[rt], fac[0], fac[2], fac[1], fac[3], w[rt].m, w[rt].L, pk[rt]);
+            wide_weights<KVF, F16>(s[rt], fac, w[rt].m, w[rt].L, pk[rt]);
         }
         __builtin_amdgcn_sched_barrier(0);
         wide_k<D>(rd, (cur + 2 * C::TILE) % (R * C::TILE), kw);
@@ -493,7 +492,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
     }
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = pair_sum(w[rt].L);
+        const float sum = pair_sum(w[rt].L) * (KVF == KVF_FP8 ? kSumUnit : 1.f);
         if (wrow + 32 * rt + c >= k.nrows) continue;
         const uint64_t at = uint64_t(k.seq.row0) + token[rt];
         if (a.splits > 1) {

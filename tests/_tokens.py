@@ -57,7 +57,8 @@ class Case:
     (NaN codes and scales).  `row0` rows come before the first sequence's and
     `pad` after the last one's."""
 
-    def __init__(self, seed, fmt, rows, hq, hkv, d, kv_len, q_len=None, row0=0, pad=0, spare=2, poison=True):
+    def __init__(self, seed, fmt, rows, hq, hkv, d, kv_len, q_len=None, row0=0, pad=0, spare=2, poison=True,
+                 amp=1.0):
         self.fmt, self.rows_type, self.hq, self.hkv, self.d = fmt, rows, hq, hkv, d
         self.kv_len = [int(t) for t in kv_len]
         self.single = q_len is None
@@ -73,6 +74,7 @@ class Case:
         x = torch.randn((size, 2, hkv, PAGE, d), generator=g)
         if fmt == "mxfp8":
             x = torch.where(torch.rand(x.shape, generator=g) < 0.01, x * 20, x)
+        x[:, 1] *= amp
         if fmt == "fp8":
             self.scales = finite_amax(x, (3, 4)) / 448.0
             self.data = e4m3(x / self.scales[..., None, None])
@@ -188,7 +190,8 @@ def attend(case, window, sinks, tiled, scale):
         |ds| <= (d + 4) 2^-24 (scale sum |q k| + |s| + |reference|) + 2^-22,
         both in the products and in their sum: 2 max|ds| A;
       f16 weights below 2^-14 are off by 2^-25 of the row's reference weight,
-        which is at most its sum: 2^-25 (1 + 1 / scale of V) sum |v|;
+        which is at most its sum: 2^-25 sum |v|; in FP8 weights have V's scale
+        in them, and so has the reference: 2^-25 sum |v| (largest / own scale);
       the sums of the products, f32: (T + 8) 2^-24 A;
       the result rounded: u |out| + the type's least step."""
     vals = values(case.data, case.scales, case.fmt)
@@ -211,10 +214,12 @@ def attend(case, window, sinks, tiled, scale):
             see = see & ((j > p - window) | (j < sinks))
         any_ = see.any(0)
         k, v = torch.where(any_[:, None, None], k, 0.0), torch.where(any_[:, None, None], v, 0.0)
-        small = torch.zeros(t, case.hkv, dtype=torch.float64)
+        small = torch.ones(t, case.hkv, dtype=torch.float64)
         if case.fmt == "fp8":
             ids = case.tables[b][:(t + PAGE - 1) // PAGE].long().clamp(0, case.data.shape[0] - 1)
-            small = (1 / case.scales[ids, 1].double()).repeat_interleave(PAGE, 0)[:t]
+            vs = torch.nan_to_num(case.scales[ids, 1].double(), 0, 0, 0)
+            small = (vs.amax(0) / vs.clamp(min=FLOOR)).repeat_interleave(PAGE, 0)[:t]
+            log = (vs.clamp(min=FLOOR).log2().abs().amax(0) + 2) * 2.0 ** -23
         for h in range(case.hq):
             g = h % case.hkv if tiled else h // (case.hq // case.hkv)
             s = q[:, h] @ k[:, g].t() * scale
@@ -227,9 +232,11 @@ def attend(case, window, sinks, tiled, scale):
             f = 2 * u + 2 * (ds + 2.0 ** -22) + (t + 8) * 2.0 ** -24
             if case.rows_type == "f32":
                 f = f - 2 * u
+            if case.fmt == "fp8":
+                f = f + 2 * float(log[g])
             e = f * A + u * o.abs()
             if case.rows_type == "f16":
-                e = e + 2.0 ** -25 * (see.double() @ (v[:, g].abs() * (1 + torch.nan_to_num(small[:, g], 0, 0, 0))[:, None]))
+                e = e + 2.0 ** -25 * (see.double() @ (v[:, g].abs() * small[:, g][:, None]))
             bound[r:r + m, h] = e + float(torch.finfo(kind).smallest_normal) * float(torch.finfo(kind).eps)
     return out, bound
 

@@ -75,6 +75,20 @@ def test_attend(backend, rows, fmt, d, shape):
     check(backend, case, window, sinks, tiled, max_kv_len=max(kv))
 
 
+@pytest.mark.parametrize("rows", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("shape", ["single-window", "short", "chunk"])
+@pytest.mark.parametrize("amp", [2.0 ** -12, 2.0 ** 12])
+def test_value_scales(backend, rows, d, shape, amp):
+    """Weights keep their 16 bits whatever V's block scales are, though a scale
+    is multiplied into them."""
+    if rows == "f16" and amp > 1:
+        amp = 2.0 ** 8          # the result has to stay in f16
+    kv, q, window, sinks, tiled = SHAPES[shape]
+    case = T.Case(41, "fp8", rows, 8, 2, d, kv, q, row0=0 if q is None else 2, pad=3, amp=amp)
+    check(backend, case, window, sinks, tiled, max_kv_len=max(kv))
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (8, 8), (5, 5), (12, 4), (40, 2), (7, 1)])
 @pytest.mark.parametrize("rows,fmt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "fp8")])
 def test_heads(backend, hq, hkv, rows, fmt):
