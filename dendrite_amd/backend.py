@@ -159,24 +159,37 @@ class TokenTables:
         c.q_indptr = None if q_indptr is None else q_indptr.data_ptr()
         c.batch_size, c.num_indices, c.max_kv_len = self.batch_size, indices.numel(), self.max_kv_len
         self._c = c
-        self._last = (-1, c)      # rows of the last call and their struct, never changed once made
+        self._last = (-1, c, None)    # rows of the last call, their struct (never changed once made), its reference
 
     def to_c(self, rows: int) -> _lib.dh_token_tables:
-        last, c = self._last
-        if last != rows:
-            c = _lib.dh_token_tables()
-            C.pointer(c)[0] = self._c
-            c.rows = rows
-            self._last = (rows, c)
-        return c
+        self.ref(rows)
+        return self._last[1]
+
+    def ref(self, rows: int):
+        """byref(to_c(rows))."""
+        last = self._last
+        if last[0] == rows:
+            return last[2]
+        c = _lib.dh_token_tables()
+        C.pointer(c)[0] = self._c
+        c.rows = rows
+        self._last = (rows, c, C.byref(c))
+        return self._last[2]
+
+
+_INT32 = None         # torch.int32
 
 
 def _status_ptr(status, device: int):
+    global _INT32
     if status is None:
         return None
-    if status.dtype is not _torch().int32 or status.numel() < 1:
+    if _INT32 is None:
+        _INT32 = _torch().int32
+    if status.dtype is not _INT32 or status.numel() < 1:
         raise DhError(_lib.DH_EINVAL, "status must be an int32 tensor")
-    _on_device(status, device, "status")
+    if status.get_device() != device:
+        _on_device(status, device, "status")
     return status.data_ptr()
 
 
@@ -194,7 +207,7 @@ class AttentionConfig:
         self.gqa_mapping = _lib.GQA_TILED         # ReferenceBackend's Tensor::repeat
         self.q_dtype = _lib.DTYPE_BF16
         self.kv_format = _lib.KV_BF16
-        self._last = (None, None)                 # fields of the last _shared_c() and its struct
+        self._last = (None, None, None)           # fields of the last _ref(), its struct and reference
 
     @classmethod
     def new(cls, num_heads: int, num_kv_heads: int, head_dim: int) -> "AttentionConfig":
@@ -221,15 +234,16 @@ class AttentionConfig:
         c.kv_format = self.kv_format
         return c
 
-    def _shared_c(self) -> _lib.dh_attn_config:
-        """to_c(), made again only when a field has changed; for reading."""
+    def _ref(self):
+        """byref(to_c()), made again only when a field has changed; for reading."""
         key = (self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.sliding_window, self.gqa_mapping,
                self.q_dtype, self.kv_format)
-        last, c = self._last
-        if last != key:
-            c = self.to_c()
-            self._last = (key, c)
-        return c
+        last = self._last
+        if last[0] == key:
+            return last[2]
+        c = self.to_c()
+        self._last = (key, c, C.byref(c))
+        return self._last[2]
 
 
 class Backend:
@@ -344,13 +358,16 @@ class Pool:
             raise DhError(_lib.DH_EINVAL, f"tables are on cuda:{tables.device}, the pool on cuda:{dev}")
         if k.dtype is not v.dtype or k.shape != v.shape:
             raise DhError(_lib.DH_EINVAL, f"k is {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
-        ks = _rows(k, self.num_kv_heads, self.head_dim, dev, "k")
-        vs = _rows(v, self.num_kv_heads, self.head_dim, dev, "v")
+        ks = vs = _rows(k, self.num_kv_heads, self.head_dim, dev, "k")
+        if v.stride() != k.stride() or v.get_device() != dev:
+            vs = _rows(v, self.num_kv_heads, self.head_dim, dev, "v")
         code = _code(k)
         if code is None:
             raise DhError(_lib.DH_EINVAL, f"row dtype {k.dtype} (float32, bfloat16 or float16)")
-        check(call(self._h, C.byref(tables.to_c(k.shape[0])), k.data_ptr(), v.data_ptr(), ks, vs, code,
-                   _status_ptr(status, dev), _device_stream(stream, dev)))
+        rc = call(self._h, tables.ref(k.shape[0]), k.data_ptr(), v.data_ptr(), ks, vs, code, _status_ptr(status, dev),
+                  _device_stream(stream, dev))
+        if rc:
+            check(rc)
 
     def append_tokens(self, tables: "TokenTables", k, v, status=None, stream=None) -> None:
         """Writes the new tokens' K and V (rows [rows, num_kv_heads, head_dim]
@@ -594,15 +611,19 @@ def attend_window(backend: Backend, pool: Pool, config: AttentionConfig, tables:
                       f"config's {torch_dtype(config.q_dtype)}")
     if sinks < 0:
         raise DhError(_lib.DH_EINVAL, f"sinks {sinks} is negative")
-    qs = _rows(q, config.num_heads, config.head_dim, dev, "q")
-    os_ = _rows(out, config.num_heads, config.head_dim, dev, "out")
+    qs = os_ = _rows(q, config.num_heads, config.head_dim, dev, "q")
+    if out.stride() != q.stride() or out.get_device() != dev:
+        os_ = _rows(out, config.num_heads, config.head_dim, dev, "out")
     ws, nbytes = None, 0
     if workspace is not None:
-        _on_device(workspace, dev, "workspace")
-        ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    check(lib().dh_attend_window(backend._h, pool._h, C.byref(config._shared_c()), min(sinks, 0xFFFFFFFF),
-                                 C.byref(tables.to_c(q.shape[0])), q.data_ptr(), qs, out.data_ptr(), os_, ws, nbytes,
-                                 _status_ptr(status, dev), _device_stream(stream, dev)))
+        if workspace.get_device() != dev:
+            _on_device(workspace, dev, "workspace")
+        ws, nbytes = workspace.data_ptr(), workspace.nbytes
+    rc = lib().dh_attend_window(backend._h, pool._h, config._ref(), min(sinks, 0xFFFFFFFF), tables.ref(q.shape[0]),
+                                q.data_ptr(), qs, out.data_ptr(), os_, ws, nbytes, _status_ptr(status, dev),
+                                _device_stream(stream, dev))
+    if rc:
+        check(rc)
 
 
 class TreeDecoder:
