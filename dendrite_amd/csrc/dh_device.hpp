@@ -265,8 +265,9 @@ constexpr int kRingShift = 7;
 constexpr uint32_t kRingRows = 1u << kRingShift, kRingMaxPages = 2048, kWideMaxPages = 384;
 // Parts that are merged 16 rows a workgroup; more are merged one row a
 // workgroup (16384 rows in 3 parts: 5 us against 26; 32 rows in 31: 12 against
-// 4; 2048 in 15: 8.5 against 6).
-constexpr uint32_t kMergeFew = 8;
+// 4; 2048 in 15: 8.5 against 6), or beyond the second number several
+// workgroups a row.
+constexpr uint32_t kMergeFew = 8, kMergeMany = 64;
 DH_HOST_DEVICE constexpr uint32_t wide_rows(uint32_t head_dim) { return head_dim == 64 ? 256u : 128u; }
 
 // Byte offset of the (page, plane, kv head) 16 x D block in the pool.

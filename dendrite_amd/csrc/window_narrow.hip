@@ -477,17 +477,20 @@ __global__ __launch_bounds__(256) void window_merge_few_kernel(WindowArgs a) {
     }
 }
 
-// Joins many parts of split work, one row a workgroup: D / 4 lanes take a part's
-// O (four elements each), the workgroup's 1024 / D lane groups every so many
-// parts; their sums are added in LDS in a fixed order.
-template <int D, uint32_t QT>
-__global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
-    constexpr int LPP = D / 4, G = 256 / LPP;
-    __shared__ float red[4];
+// Joins many parts of split work, COLS columns of a row a workgroup: COLS / 4
+// lanes take a part's (four elements each), the workgroup's lane groups every so
+// many parts; their sums are added in LDS in a fixed order.  Whole rows and 256
+// threads; beyond kMergeMany parts, of few rows, 64 columns and 1024 threads have
+// all loads in flight at once (16 rows of 256 dims in 256 parts: 5.8 us, and
+// 10.2 by whole rows; 3840 rows of 128 in a dozen: 15 by 64 columns, and 9.9).
+template <int D, uint32_t QT, int COLS, int NT>
+__global__ __launch_bounds__(NT) void window_merge_kernel(WindowArgs a) {
+    constexpr int CB = D / COLS, LPP = COLS / 4, G = NT / LPP;
+    __shared__ float red[NT / 64];
     __shared__ __attribute__((aligned(16))) f4 acc[G][LPP];
     __shared__ float sums[G];
-    const uint32_t x0 = blockIdx.x >> 4, unit = x0 / a.hkv;
-    const int row = int(blockIdx.x & 15);
+    const uint32_t x0 = blockIdx.x / (16 * CB), unit = x0 / a.hkv;
+    const int row = int(blockIdx.x / CB & 15), cb = int(blockIdx.x % CB);
     const RowBlock k = find_rows<4>(a, unit, int(x0 - unit * a.hkv));
     if (row >= k.nrows) return;
     const int tid = threadIdx.x;
@@ -497,13 +500,15 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
     const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
     const int splits = k.zero ? 0 : int(a.splits);
     float mx = kNegInf;
-    for (int s = tid; s < splits; s += 256) mx = fmaxf(mx, ml[s][0]);
+    for (int s = tid; s < splits; s += NT) mx = fmaxf(mx, ml[s][0]);
     #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
     if ((tid & 63) == 0) red[tid >> 6] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const int grp = tid / LPP, col = tid % LPP;
+    mx = red[0];
+    #pragma unroll
+    for (int i = 1; i < NT / 64; ++i) mx = fmaxf(mx, red[i]);
+    const int grp = tid / LPP, col = cb * LPP + tid % LPP;
     f4 x = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
     #pragma unroll 4
@@ -513,15 +518,15 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WindowArgs a) {
         sum += al * v[1];
         x += reinterpret_cast<const f4*>(a.ws_o + (slot + s) * D)[col] * al;
     }
-    acc[grp][col] = x;
-    if (col == 0) sums[grp] = sum;
+    acc[grp][tid % LPP] = x;
+    if (tid % LPP == 0) sums[grp] = sum;
     __syncthreads();
     if (tid >= LPP) return;
-    x = acc[0][col];
+    x = acc[0][tid];
     sum = sums[0];
     #pragma unroll
     for (int g = 1; g < G; ++g) {
-        x += acc[g][col];
+        x += acc[g][tid];
         sum += sums[g];
     }
     write_merged<D, QT>(a, at, head, col, x, sum);
@@ -564,8 +569,10 @@ template <int D, uint32_t QT>
 void launch_merge_q(const WindowArgs& a, uint32_t blocks, hipStream_t s) {
     if (a.splits <= kMergeFew)
         hipLaunchKernelGGL((window_merge_few_kernel<D, QT>), dim3(blocks), dim3(256), 0, s, a);
+    else if (a.splits <= kMergeMany)
+        hipLaunchKernelGGL((window_merge_kernel<D, QT, D, 256>), dim3(blocks * 16), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((window_merge_kernel<D, QT>), dim3(blocks * 16), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((window_merge_kernel<D, QT, 64, 1024>), dim3(blocks * (16 * (D / 64))), dim3(1024), 0, s, a);
 }
 
 template <int D>
@@ -596,7 +603,7 @@ int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, ui
 
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream) {
     const uint64_t blocks = row_blocks(a, 4) * a.hkv;
-    if (blocks > 0x7FFFFFFull) return hipErrorInvalidValue;
+    if (blocks > 0x1FFFFFFull) return hipErrorInvalidValue;
     const uint32_t grid = uint32_t(blocks);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (d) {
