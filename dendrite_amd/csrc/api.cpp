@@ -1331,6 +1331,7 @@ dh_status token_copy(const dh_pool* p, const dh_token_tables* t, const void* k, 
     a.scales = p->scales;
     a.num_pages = p->num_pages;
     a.hkv = p->hkv;
+    a.by_planes = dh::Divisor::of(2 * p->hkv);
     a.status = status;
     const hipError_t e = hipError_t(append ? dh::launch_append_tokens(a, dtype, p->fmt, p->d, stream)
                                            : dh::launch_read_tokens(a, dtype, p->fmt, p->d, stream));
@@ -1494,6 +1495,9 @@ dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_co
     a.sinks = int32_t(w.sinks);
     a.page_limit = pool->num_pages;
     a.splits = w.splits;
+    a.by_hkv = dh::Divisor::of(a.hkv);
+    a.by_r = dh::Divisor::of(r);
+    a.by_splits = dh::Divisor::of(w.splits);
     a.status = status;
     hipError_t e = hipError_t(
         !w.wide  ? dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, w.waves, stream)

@@ -225,6 +225,20 @@ struct TokenTables {
     uint32_t batch, num_indices, rows, max_kv_len;
 };
 
+// Division of n < 2^31 by a number the host knows: n mul >> shift with mul =
+// ceil(2^shift / d), shift = 31 + ceil(log2 d); mul d exceeds 2^shift by less than
+// 2^(shift - 31), so the quotient is exact (Granlund and Montgomery).  The GPU
+// has no integer division: the compiler's takes some 35 instructions.
+struct Divisor {
+    uint32_t mul, shift;
+    static Divisor of(uint32_t d) {
+        uint32_t s = 31;
+        while ((1ull << (s - 31)) < d) ++s;
+        return {uint32_t(((1ull << s) + d - 1) / d), s};
+    }
+    DH_HOST_DEVICE uint32_t operator()(uint32_t n) const { return uint32_t(uint64_t(n) * mul >> shift); }
+};
+
 struct TokenCopyArgs {
     TokenTables t;
     uint8_t* k;                  // rows: read by append, written by read
@@ -233,6 +247,7 @@ struct TokenCopyArgs {
     uint8_t* data;
     uint8_t* scales;
     uint32_t num_pages, hkv;
+    Divisor by_planes;           // 2 hkv
     int32_t* status;
 };
 
@@ -251,6 +266,7 @@ struct WindowArgs {
     int32_t window, sinks;       // window 0: none (sinks then 0)
     uint32_t page_limit;
     uint32_t splits;             // >= 1; 1: the attention kernel writes out
+    Divisor by_hkv, by_r, by_splits;
     int32_t* status;
 };
 

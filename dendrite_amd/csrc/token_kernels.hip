@@ -135,7 +135,7 @@ __device__ __forceinline__ Block find_block(const TokenCopyArgs& a) {
     Block k{};
     const uint32_t per = 2 * a.hkv;
     const uint32_t item = blockIdx.x * 4 + uint32_t(uniform(threadIdx.x >> 6));
-    const uint32_t unit = item / per, ph = item - unit * per;
+    const uint32_t unit = a.by_planes(item), ph = item - unit * per;
     k.plane = ph >= a.hkv ? 1u : 0u;
     k.head = ph - k.plane * a.hkv;
     uint32_t u = 0;
@@ -313,7 +313,7 @@ uint64_t token_units(const TokenTables& t) {
 template <bool APPEND, int D, uint32_t ROW, uint32_t FMT>
 hipError_t launch_one(const TokenCopyArgs& a, hipStream_t s) {
     const uint64_t blocks = (token_units(a.t) * 2 * a.hkv + 3) / 4;
-    if (blocks > 0x3FFFFFFFull) return hipErrorInvalidValue;     // four items a workgroup in 32 bits
+    if (blocks > 0x1FFFFFFFull) return hipErrorInvalidValue;     // four items a workgroup in 31 bits
     if constexpr (APPEND)
         hipLaunchKernelGGL((append_tokens_kernel<D, ROW, FMT>), dim3(uint32_t(blocks)), dim3(256), 0, s, a);
     else

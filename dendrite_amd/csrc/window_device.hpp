@@ -35,7 +35,7 @@ __device__ __forceinline__ RowBlock find_rows(const WindowArgs& a, uint64_t unit
     } else {
         const uint32_t per = (a.r + (1u << SHIFT) - 1) >> SHIFT;
         if (unit >= uint64_t(a.t.batch) * per) return k;
-        const uint32_t b = uint32_t(unit) / per;
+        const uint32_t b = per == 1 ? uint32_t(unit) : uint32_t(unit) / per;
         u = uint32_t(unit) - b * per;
         k.seq = uniform_sequence(load_sequence(a.t, b));
     }
@@ -46,8 +46,8 @@ __device__ __forceinline__ RowBlock find_rows(const WindowArgs& a, uint64_t unit
     k.zero = !k.seq.ok || k.seq.n == 0;
     if (k.zero) return k;
     const int first = k.seq.len - k.seq.n;
-    k.pmin = first + k.rho0 / int(a.r);
-    k.pmax = first + (k.rho0 + k.nrows - 1) / int(a.r);
+    k.pmin = first + int(a.by_r(k.rho0));
+    k.pmax = first + int(a.by_r(k.rho0 + k.nrows - 1));
     const int lo = a.window ? max(0, k.pmin - a.window + 1) : 0;
     k.window_page = lo >> 4;
     k.sink_pages = a.window ? min((min(a.sinks, k.pmax + 1) + 15) >> 4, k.window_page) : 0;
@@ -80,7 +80,7 @@ __device__ __forceinline__ int list_page(const RowBlock& k, int j) {
 
 // Row rho's offset (in rows of q / out) and query head.
 __device__ __forceinline__ void row_place(const WindowArgs& a, const RowBlock& k, int rho, int& token, int& head) {
-    token = rho / int(a.r);
+    token = int(a.by_r(rho));
     const int j = rho - token * int(a.r);
     head = a.tiled ? k.kv_head + j * int(a.hkv) : k.kv_head * int(a.r) + j;
 }

@@ -25,8 +25,10 @@ struct WavePages {
     int id[kNarrowWavePages / 64];
     int j0, n;      // first list entry, entries
 
-    __device__ __forceinline__ void load(const WindowArgs& a, const RowBlock& k, int part, int parts) {
-        int per = uniform((k.pages + parts - 1) / parts);
+    // Part `part` of a.splits NW.
+    template <int NW>
+    __device__ __forceinline__ void load(const WindowArgs& a, const RowBlock& k, int part) {
+        int per = uniform(int(a.by_splits(uint32_t(k.pages) + a.splits * NW - 1) / NW));
         per += per & 1;
         j0 = min(part * per, k.pages);
         n = min(min(per, k.pages - j0), int(kNarrowWavePages));
@@ -131,9 +133,9 @@ __device__ __forceinline__ void join_waves(const WindowArgs& a, const RowBlock& 
 template <int SHIFT>
 __device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& split) {
     const bool refused = sees_refused(a.t, blockIdx.x);
-    const uint32_t x = blockIdx.x / a.hkv;
+    const uint32_t x = a.by_hkv(blockIdx.x);
     const int head = uniform(int(blockIdx.x - x * a.hkv));
-    const uint32_t unit = x / a.splits;
+    const uint32_t unit = a.by_splits(x);
     split = uniform(int(x - unit * a.splits));
     const RowBlock k = uniform_block(find_rows<SHIFT>(a, unit, head));
     report(refused, a.status);
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     WavePages pages;
-    pages.load(a, k, split * NW + wave, int(a.splits) * NW);
+    pages.load<NW>(a, k, split * NW + wave);
 
     // Query rows as B operands: lane (g, c) holds row c.
     const int rho = k.rho0 + min(c, k.nrows - 1);
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) 
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     WavePages pages;
-    pages.load(a, k, split * NW + wave, int(a.splits) * NW);
+    pages.load<NW>(a, k, split * NW + wave);
     const int rho = k.rho0 + min(c, k.nrows - 1);
     int token, head;
     row_place(a, k, rho, token, head);
@@ -452,7 +454,7 @@ __device__ __forceinline__ void write_merged(const WindowArgs& a, uint64_t at, i
 template <int D, uint32_t QT>
 __global__ __launch_bounds__(256) void window_merge_few_kernel(WindowArgs a) {
     constexpr int LPP = D / 4, G = 256 / LPP;
-    const uint32_t unit = blockIdx.x / a.hkv;
+    const uint32_t unit = a.by_hkv(blockIdx.x);
     const RowBlock k = find_rows<4>(a, unit, int(blockIdx.x - unit * a.hkv));
     const int grp = threadIdx.x / LPP, col = threadIdx.x % LPP;
     const int splits = k.zero ? 0 : int(a.splits);
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(NT) void window_merge_kernel(WindowArgs a) {
     __shared__ float red[NT / 64];
     __shared__ __attribute__((aligned(16))) f4 acc[G][LPP];
     __shared__ float sums[G];
-    const uint32_t x0 = blockIdx.x / (16 * CB), unit = x0 / a.hkv;
+    const uint32_t x0 = blockIdx.x / (16 * CB), unit = a.by_hkv(x0);
     const int row = int(blockIdx.x / CB & 15), cb = int(blockIdx.x % CB);
     const RowBlock k = find_rows<4>(a, unit, int(x0 - unit * a.hkv));
     if (row >= k.nrows) return;

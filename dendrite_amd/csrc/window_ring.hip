@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
     __shared__ __attribute__((aligned(1024))) uint8_t ring[C::RING];
     __shared__ int ids[kRingMaxPages + 2 * (P + 1)];
     const bool refused = sees_refused(a.t, blockIdx.x);
-    const uint32_t x0 = blockIdx.x / a.hkv;
-    const uint32_t unit = x0 / a.splits;
+    const uint32_t x0 = a.by_hkv(blockIdx.x);
+    const uint32_t unit = a.by_splits(x0);
     const int split = uniform(int(x0 - unit * a.splits));
     const RowBlock k = uniform_block(find_rows<kRingShift>(a, unit, int(blockIdx.x - x0 * a.hkv)));
     report(refused, a.status);
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
         return;
     }
     // This workgroup's part of the page list, whole pairs.
-    int per = uniform((k.pages + int(a.splits) - 1) / int(a.splits));
+    int per = uniform(int(a.by_splits(uint32_t(k.pages) + a.splits - 1)));
     per += per & 1;
     const int j0 = min(split * per, k.pages), n = min(min(per, k.pages - j0), int(kRingMaxPages));
     const uint32_t npairs = uint32_t(n + 1) >> 1;
@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
     int seen0 = 0, seen1 = 0;
     if (!holes) {
         const int last = k.nrows - 1;
-        const int wmin = first + (k.rho0 + min(wave * kTileRows, last)) / int(a.r);
-        const int wmax = first + (k.rho0 + min(((RT - 1) * kWaves + wave) * kTileRows + kTileRows - 1, last)) / int(a.r);
+        const int wmin = first + int(a.by_r(k.rho0 + min(wave * kTileRows, last)));
+        const int wmax = first + int(a.by_r(k.rho0 + min(((RT - 1) * kWaves + wave) * kTileRows + kTileRows - 1, last)));
         const int lo = a.window ? max(wmax - a.window + 1, 0) : 0;
         seen0 = k.sink_pages + max(((lo + 15) >> 4) - k.window_page, 0) - j0;
         seen1 = min(n, k.sink_pages + ((wmin + 1) >> 4) - k.window_page - j0);

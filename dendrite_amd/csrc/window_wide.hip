@@ -334,8 +334,8 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
     __shared__ int ids[kWideMaxPages + (C::RING + C::AHEAD + 2) * NP];        // (read ahead)
     __shared__ __attribute__((aligned(16))) f2 scl[KVF == KVF_FP8 ? kWideMaxPages + 2 * NP : 1];
     const bool refused = sees_refused(a.t, blockIdx.x);
-    const uint32_t x0 = blockIdx.x / a.hkv;
-    const uint32_t unit = x0 / a.splits;
+    const uint32_t x0 = a.by_hkv(blockIdx.x);
+    const uint32_t unit = a.by_splits(x0);
     const int split = uniform(int(x0 - unit * a.splits));
     const RowBlock k = uniform_block(find_rows<C::SHIFT>(a, unit, int(blockIdx.x - x0 * a.hkv)));
     report(refused, a.status);
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
         return;
     }
     // This workgroup's part of the page list, whole tiles.
-    int per = uniform((k.pages + int(a.splits) - 1) / int(a.splits));
+    int per = uniform(int(a.by_splits(uint32_t(k.pages) + a.splits - 1)));
     per = (per + NP - 1) / NP * NP;
     const int j0 = min(split * per, k.pages), n = min(min(per, k.pages - j0), int(kWideMaxPages));
     const int ntiles = (n + NP - 1) / NP;
@@ -384,8 +384,8 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
         #pragma unroll
         for (int kb = 0; kb < KB; ++kb) q[rt][kb] = *reinterpret_cast<const u32x4*>(qp + 32 * kb) ^ a.q_sign;
     }
-    const int wmin = uniform(first + (k.rho0 + min(wrow, k.nrows - 1)) / int(a.r));
-    const int wmax = uniform(first + (k.rho0 + min(wrow + 32 * RT - 1, k.nrows - 1)) / int(a.r));
+    const int wmin = uniform(first + int(a.by_r(k.rho0 + min(wrow, k.nrows - 1))));
+    const int wmax = uniform(first + int(a.by_r(k.rho0 + min(wrow + 32 * RT - 1, k.nrows - 1))));
     WideRows<D> w[RT];
     #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
