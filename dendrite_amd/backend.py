@@ -234,6 +234,9 @@ class AttentionConfig:
         c.kv_format = self.kv_format
         return c
 
+    def __getstate__(self):
+        return dict(self.__dict__, _last=(None, None, None))     # (a reference cannot be copied)
+
     def _ref(self):
         """byref(to_c()), made again only when a field has changed; for reading."""
         key = (self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.sliding_window, self.gqa_mapping,

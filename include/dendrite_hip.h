@@ -567,7 +567,8 @@ size_t dh_window_workspace_size(const dh_attn_config* cfg, const dh_token_tables
  * DH_INVALID_PAGE.  The K / V of the new tokens are expected in the pages
  * (dh_pool_append_tokens before).  Slots past kv_len may hold anything; a NaN
  * or infinity among a sequence's own V reaches the rows that see it and may
- * reach the sequence's other rows of the call.
+ * reach the sequence's other rows of the call.  An FP8 block scale of V below
+ * 2^-64, the least dh_pool_append_tokens writes, counts as 2^-64.
  *   q, out    : device, row i at q + i * q_stride elements of cfg->q_dtype,
  *               [num_heads][head_dim] each; strides >= num_heads * head_dim,
  *               rows and strides multiples of 16 bytes; out overlaps nothing

@@ -89,6 +89,15 @@ def test_value_scales(backend, rows, d, shape, amp):
     check(backend, case, window, sinks, tiled, max_kv_len=max(kv))
 
 
+@pytest.mark.parametrize("shape", ["single-window", "short", "chunk"])
+@pytest.mark.parametrize("amp", [2.0 ** -50, 2.0 ** 100])
+def test_extreme_value_scales(backend, shape, amp):
+    """The row's sum takes V's scales out again: it stays within f32."""
+    kv, q, window, sinks, tiled = SHAPES[shape]
+    case = T.Case(42, "fp8", "bf16", 8, 2, 128, kv, q, row0=0 if q is None else 2, pad=3, amp=amp)
+    check(backend, case, window, sinks, tiled, max_kv_len=max(kv))
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (8, 8), (5, 5), (12, 4), (40, 2), (7, 1)])
 @pytest.mark.parametrize("rows,fmt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "fp8")])
 def test_heads(backend, hq, hkv, rows, fmt):

@@ -1,6 +1,7 @@
 """The token operators without a GPU: the plain forms the GPU tests compare
 with against the decode oracle, workspace sizes, and refusals that need no
 device."""
+import copy
 import ctypes as C
 
 import numpy as np
@@ -63,6 +64,17 @@ def test_workspace_size():
     assert size(1, 1, 131072, True) < small
     assert L.dh_window_workspace_size(None, C.byref(_tables(1, 1, 1, True)), 0) == 0
     assert L.dh_window_workspace_size(C.byref(cfg), None, 0) == 0
+
+
+def test_configs_are_copied_after_use():
+    cfg = AttentionConfig(32, 8, 128)
+    first = cfg._ref()
+    assert cfg._ref() is first
+    other = copy.deepcopy(cfg)
+    other.sliding_window = 5
+    assert other._ref()._obj.sliding_window == 5 and cfg._ref() is first and first._obj.sliding_window == 0
+    cfg.scale = 2.0
+    assert cfg._ref()._obj.scale == 2.0
 
 
 def test_null_handles_are_refused():
