@@ -10,8 +10,14 @@
 // with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32 (16x16x4 for
 // f32), operands straight from global memory (attend_device.hpp's layout).
 // The waves' states are joined in LDS; with several parts each workgroup
-// writes (O, m, L) in f32 and window_merge_kernel joins them.  Bound by the
-// cache's bytes: every page is read once per block.
+// writes (O, m, L) in f32 and a merge kernel joins them.
+//
+// Every page is read once per block.  Large batches are bound by those bytes (64
+// sequences under a window of 4096, bf16, 32 heads of 128: 166 us, 5.6 TB/s; 256
+// in FP8 under 1024 + 64, 64 heads: 109 us, 4.7; one token over 100 000, f16, 16
+// heads of 256: 38 us, 5.3), blocks of several tokens by 8-bit conversion (32
+// sequences of 3 to 9 tokens in MXFP8, 16 heads of 256: 42 us), small calls by
+// their dependent loads (one f32 token under a window of 256: 9.1 us).
 #include "attend_device.hpp"
 #include "window_device.hpp"
 
