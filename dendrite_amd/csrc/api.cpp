@@ -1403,22 +1403,27 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     // split (one sequence of 512 tokens, window 256, f32: 9.7 us, and 11.1 with
     // four waves), or blocks that fill half the chip (64 sequences of 5000 tokens
     // in FP8, 4 KV heads of 64: 32 us, and 41 with four waves in two parts), in
-    // 8-bit caches all of it (70 sequences: 46 us, and 65; but 90 and 79 in bf16).
+    // 8-bit caches all of it (70 sequences: 46 us, and 65; but 90 and 79 in bf16),
+    // and are not short lists with blocks of no rows among them (32 sequences of
+    // 3 tokens under a window of 2001, 4 KV heads of 64, bf16: 32 us with eight
+    // waves, and 27 with four in two parts; FP8: 29 with 16, 25 with eight).
     // Long lists of few blocks are faster in parts on many CUs (one sequence of
     // 5000 tokens: 13 us, and 18 with 16 waves).
+    // blocks that have rows: one a sequence at least, its last one part empty
+    const uint64_t some = (rows + t.batch_size * block / 2 + block / 2 - 1) / block;
+    const uint64_t filled = t.q_indptr ? std::max<uint64_t>(t.batch_size, some) * c.num_kv_heads : blocks;
+    const uint64_t waves = dh::narrow_waves(c.head_dim, codes);
     w.waves = dh::kWaves;
-    while (2 * w.waves <= dh::narrow_waves(c.head_dim) && 2 * w.waves * blocks <= 256 * dh::narrow_waves(c.head_dim) &&
-           (blocks > 128 || pages < 32) && (blocks <= 256 || codes))
+    while (2 * w.waves <= waves && 2 * w.waves * filled <= 256 * waves && (filled <= 256 || codes) &&
+           (filled > 128 ? !t.q_indptr || pages * c.head_dim >= (codes ? 12 : 24) * 128 * w.waves : pages < 32))
         w.waves *= 2;
     const uint64_t cap = !w.wide ? w.waves * (dh::kNarrowWavePages - 2)
                                  : (w.ring ? dh::kRingMaxPages : dh::kWideMaxPages) - 8;
     const uint64_t least = std::max<uint64_t>(1, (pages + cap - 1) / cap);
     if (w.wide) {
-        // blocks that have rows: one a sequence may be part empty
-        const uint64_t filled = (rows + t.batch_size * block / 2 + block / 2 - 1) / block * c.num_kv_heads;
         w.splits = wide_splits(c, w.ring, uint64_t(t.rows) * c.num_heads, filled, pages, least);
     } else {
-        const uint64_t want = 2048 / w.waves / std::max<uint64_t>(1, blocks);
+        const uint64_t want = 2048 / w.waves / std::max<uint64_t>(1, filled);
         w.splits = uint32_t(std::max(least, std::min(want, pages / (4 * w.waves))));
     }
     if (w.splits > 1) {

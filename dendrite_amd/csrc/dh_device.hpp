@@ -275,8 +275,10 @@ struct WindowArgs {
 // a narrow block and a wide block may be given (registers, LDS lists).
 constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256;
 // Most waves of a narrow workgroup, as the registers allow (D = 64: 128 a wave,
-// D = 128: 256).
-DH_HOST_DEVICE constexpr uint32_t narrow_waves(uint32_t head_dim) { return head_dim == 64 ? 16u : head_dim == 128 ? 8u : 4u; }
+// D = 128, and 256 over 8-bit pages: 256).
+DH_HOST_DEVICE constexpr uint32_t narrow_waves(uint32_t head_dim, bool codes) {
+    return head_dim == 64 ? 16u : head_dim == 128 || codes ? 8u : 4u;
+}
 constexpr int kRingShift = 7;
 constexpr uint32_t kRingRows = 1u << kRingShift, kRingMaxPages = 2048, kWideMaxPages = 384;
 // Parts that are merged 16 rows a workgroup; more are merged one row a

@@ -1,10 +1,10 @@
 // Windowed attention of few query rows a sequence, from device tables: single
 // tokens and short chunks (dh_attend_window), and the merge of split work.
 //
-// A workgroup of four waves has one block of 16 rows (one MFMA tile) of one KV
-// head and one of `splits` equal parts of the block's page list; each wave
-// takes a quarter of the part, a pair of pages (32 tokens) at a time, with the
-// loads of the next pair in flight behind the math of the current one:
+// A workgroup of 4, 8 or 16 waves has one block of 16 rows (one MFMA tile) of
+// one KV head and one of `splits` equal parts of the block's page list; each
+// wave takes its share of the part, a pair of pages (32 tokens) at a time, with
+// the loads of the next pair in flight behind the math of the current one:
 //   s = scale q K^T, m' = max(m, max s), O = O 2^(m - m') + 2^(s - m') V,
 //   L = L 2^(m - m') + sum 2^(s - m')   (s in log2 units)
 // with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32 (16x16x4 for
@@ -543,13 +543,7 @@ __global__ __launch_bounds__(NT) void window_merge_kernel(WindowArgs a) {
 template <int D, int NW>
 hipError_t launch_narrow_w(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, dim3 grid, hipStream_t s) {
     const dim3 block(64 * NW);
-    if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32)
-        hipLaunchKernelGGL((window_narrow32_kernel<D, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_BF16)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_F16)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_FP8)
+    if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_FP8)
         hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, false, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_FP8)
         hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, true, NW>), grid, block, 0, s, a);
@@ -557,19 +551,27 @@ hipError_t launch_narrow_w(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, 
         hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, false, NW>), grid, block, 0, s, a);
     else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_MX)
         hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, true, NW>), grid, block, 0, s, a);
-    else
+    else if constexpr (NW <= int(narrow_waves(D, false))) {
+        if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32)
+            hipLaunchKernelGGL((window_narrow32_kernel<D, NW>), grid, block, 0, s, a);
+        else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_BF16)
+            hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false, NW>), grid, block, 0, s, a);
+        else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_F16)
+            hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true, NW>), grid, block, 0, s, a);
+        else
+            return hipErrorInvalidValue;
+    } else {
         return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_narrow_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t waves, dim3 grid, hipStream_t s) {
-    if constexpr (narrow_waves(D) >= 16) {
+    if constexpr (narrow_waves(D, true) >= 16) {
         if (waves == 16) return launch_narrow_w<D, 16>(a, q_dtype, fmt, grid, s);
     }
-    if constexpr (narrow_waves(D) >= 8) {
-        if (waves == 8) return launch_narrow_w<D, 8>(a, q_dtype, fmt, grid, s);
-    }
+    if (waves == 8) return launch_narrow_w<D, 8>(a, q_dtype, fmt, grid, s);
     return waves == kWaves ? launch_narrow_w<D, kWaves>(a, q_dtype, fmt, grid, s) : hipErrorInvalidValue;
 }
 

@@ -13,13 +13,14 @@
 // place in the list, and the mask stands apart from the one copy of the step
 // (two copies, masked and not, took 208 registers more than there are).
 //
-// Bound by the matrix cores' clock: 4096 tokens x 64 heads of 128 dims over a
-// window of 2048 and 128 first tokens run at 0.96 PFLOP/s (294 us, bf16), where
-// a large library product reaches 1.08.  What it took, same shape: pages staged
-// through registers (window_wide.hip) 343 us; one workgroup a CU, as the two
-// copies of the step allowed, 560.  Heads of 64: three workgroups a CU (170
-// registers) 92 us at 4096 tokens x 32 heads and 35 at 12 prompts of 500, two
-// 96 and 40.
+// Bound by the matrix cores' clock: 4096 tokens over 8192, 32 heads of 128 dims,
+// window 4096, run at 1.08 to 1.15 PFLOP/s (240 to 255 us, bf16; the matrix unit
+// busy 55 % of the cycles), as a large library product does (1.08).  Pages staged
+// through registers instead (window_wide.hip) 340 us; one workgroup a CU, which
+// two copies of the step allow, 560.  Heads of 64: three workgroups a CU (168
+// registers) 92 us at 4096 tokens x 32 heads over 2048 and 35 at 12 prompts of
+// 500, two 96 and 40; short windows' blocks are bound by their start (12 prompts,
+// window 256: 52 us, 16 % busy).
 #include "attend_device.hpp"
 #include "window_device.hpp"
 
