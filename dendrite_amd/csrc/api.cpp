@@ -1346,8 +1346,13 @@ struct WindowPlan {
     uint32_t waves;            // of a narrow workgroup
     uint32_t splits;
     uint32_t window, sinks;
+    uint32_t rows;             // of a block
+    uint32_t tail, tail_blocks, tail_parts;     // wide blocks split by themselves (WindowArgs)
     size_t o_bytes, bytes;     // workspace: O, all
 };
+
+// Workgroups of a wide kernel the chip holds at once.
+uint32_t wide_slots(uint32_t head_dim, bool ring) { return head_dim == 256 ? 256 : ring && head_dim == 64 ? 768 : 512; }
 
 // Parts of a wide block's page list: the fewest microseconds by a model of the
 // wide kernels, fitted to their times.  A full chip takes head_dim / 256 us a
@@ -1358,7 +1363,7 @@ struct WindowPlan {
 // 32 284 and 243.)
 uint32_t wide_splits(const dh_attn_config& c, bool ring, uint64_t states, uint64_t blocks, uint64_t pages,
                      uint64_t least) {
-    const double slots = c.head_dim == 256 ? 256 : ring && c.head_dim == 64 ? 768 : 512;
+    const double slots = wide_slots(c.head_dim, ring);
     const double page = c.head_dim / 256.0, state = states * c.head_dim * 8 / 4.5e6;
     const uint64_t most = std::max(least, std::min<uint64_t>(pages / 16, uint64_t(2 * slots) / blocks + 1));
     uint64_t best = least;
@@ -1426,8 +1431,26 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
         const uint64_t want = 2048 / w.waves / std::max<uint64_t>(1, filled);
         w.splits = uint32_t(std::max(least, std::min(want, pages / (4 * w.waves))));
     }
-    if (w.splits > 1) {
-        const size_t states = size_t(t.rows) * c.num_heads * w.splits;
+    // A last round of few blocks, each alone on its CU with a whole list before
+    // it, in parts (a block alone takes about 0.45 of a full chip's time a page;
+    // the ring kernel at 64 dims has no register to spare for it).  1056 tokens x
+    // 64 heads of 128 over 2048: 90 us, and 111 whole (bf16), 106 and 133 (FP8);
+    // 2200 x 16 heads of 256: 140 and 200.
+    w.rows = uint32_t(block);
+    w.tail = dh::kNoTail;
+    const uint64_t slots = wide_slots(c.head_dim, w.ring), rounds = filled / slots;
+    if (w.wide && w.splits == 1 && !(w.ring && c.head_dim == 64) && rounds >= 1 && rounds <= 4 && filled > rounds * slots) {
+        const uint64_t n = blocks - rounds * slots;
+        const uint64_t parts = std::min<uint64_t>({dh::kMergeFew, slots / n, pages / 32});
+        if (parts > 1 && 0.45 * pages * c.head_dim / 256 * (parts - 1) / parts > 10) {
+            w.tail = uint32_t(rounds * slots);
+            w.tail_blocks = uint32_t(n);
+            w.tail_parts = uint32_t(parts);
+        }
+    }
+    const size_t split_states = size_t(w.tail_blocks) * block * w.tail_parts;
+    if (w.splits > 1 || split_states) {
+        const size_t states = split_states ? split_states : size_t(t.rows) * c.num_heads * w.splits;
         w.o_bytes = align256(states * c.head_dim * sizeof(float));
         w.bytes = w.o_bytes + align256(states * 2 * sizeof(float));
     }
@@ -1503,14 +1526,19 @@ dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_co
     a.by_hkv = dh::Divisor::of(a.hkv);
     a.by_r = dh::Divisor::of(r);
     a.by_splits = dh::Divisor::of(w.splits);
+    a.tail = w.tail;
+    a.tail_parts = w.tail_parts;
+    a.by_tail = dh::Divisor::of(std::max(1u, w.tail_parts));
     a.status = status;
     hipError_t e = hipError_t(
         !w.wide  ? dh::launch_window_narrow(a, c.q_dtype, c.kv_format, c.head_dim, w.waves, stream)
         : w.ring ? dh::launch_window_ring(a, c.q_dtype, c.head_dim, stream)
                  : dh::launch_window_wide(a, c.q_dtype, c.kv_format, c.head_dim, stream));
     if (e != hipSuccess) return fail(DH_EHIP, "window attention launch failed: %s", hipGetErrorString(e));
-    if (w.splits > 1) {
-        e = hipError_t(dh::launch_window_merge(a, c.q_dtype, c.head_dim, stream));
+    if (w.splits > 1 || w.tail_blocks) {
+        e = hipError_t(w.tail_blocks
+                           ? dh::launch_window_merge_tail(a, c.q_dtype, c.head_dim, w.tail_blocks, w.rows, stream)
+                           : dh::launch_window_merge(a, c.q_dtype, c.head_dim, stream));
         if (e != hipSuccess) return fail(DH_EHIP, "merge launch failed: %s", hipGetErrorString(e));
     }
     return DH_OK;

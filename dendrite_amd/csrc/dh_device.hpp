@@ -267,12 +267,18 @@ struct WindowArgs {
     uint32_t page_limit;
     uint32_t splits;             // >= 1; 1: the attention kernel writes out
     Divisor by_hkv, by_r, by_splits;
+    // Wide blocks tail, tail + 1, ... (KV heads fastest) are split tail_parts
+    // ways, the others not (splits 1); kNoTail: none.  Row i of the block, part
+    // s: state ((block - tail) rows + i) tail_parts + s of ws_o / ws_ml.
+    uint32_t tail, tail_parts;
+    Divisor by_tail;
     int32_t* status;
 };
 
 // Query rows of a narrow block (one MFMA tile), of a wide one fed through LDS
 // directly (window_ring.hip) and of one fed through registers; pages a wave of
 // a narrow block and a wide block may be given (registers, LDS lists).
+constexpr uint32_t kNoTail = 0xFFFFFFFFu;
 constexpr uint32_t kNarrowRows = 16, kNarrowWavePages = 256;
 // Most waves of a narrow workgroup, as the registers allow (D = 64: 128 a wave,
 // D = 128, and 256 over 8-bit pages: 256).
@@ -351,6 +357,8 @@ int launch_read_tokens(const TokenCopyArgs& a, uint32_t dst_dtype, uint32_t fmt,
 int launch_window_narrow(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, uint32_t waves,
                          void* stream);
 int launch_window_wide(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, uint32_t d, void* stream);
+int launch_window_merge_tail(const WindowArgs& a, uint32_t q_dtype, uint32_t d, uint32_t blocks, uint32_t rows,
+                             void* stream);
 int launch_window_ring(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void* stream);
 }  // namespace dh

@@ -73,6 +73,43 @@ __device__ __forceinline__ RowBlock uniform_block(const RowBlock& x) {
     return k;
 }
 
+// The block, and the part of its page list, of a workgroup of a wide kernel: KV
+// heads fastest (neighbouring pages' planes), then parts, then blocks.
+struct BlockPart {
+    uint32_t unit;
+    int head, split, parts;
+    uint32_t place;         // the block's in the tail (0 where there is none)
+};
+
+// TAIL: the call may have one (a.tail).
+template <bool TAIL>
+__device__ __forceinline__ BlockPart block_part(const WindowArgs& a) {
+    uint32_t x = blockIdx.x, split = 0, parts = a.splits, place = 0;
+    if (TAIL && x >= a.tail) {
+        place = a.by_tail(x - a.tail);
+        parts = a.tail_parts;
+        split = x - a.tail - place * parts;
+        x = a.tail + place;
+    }
+    const uint32_t x0 = a.by_hkv(x), unit = a.by_splits(x0);
+    return {unit, uniform(int(x - x0 * a.hkv)), uniform(int(split + x0 - unit * a.splits)), uniform(int(parts)), place};
+}
+
+// Entries of a part of the list.
+template <bool TAIL>
+__device__ __forceinline__ int part_pages(const WindowArgs& a, const BlockPart& b, int pages) {
+    const uint32_t n = uint32_t(pages) + uint32_t(b.parts) - 1;
+    return uniform(int(TAIL && blockIdx.x >= a.tail ? a.by_tail(n) : a.by_splits(n)));
+}
+
+// Where row i of the block (of `rows`), row `at` of the call, keeps its state.
+template <bool TAIL>
+__device__ __forceinline__ uint64_t state_slot(const WindowArgs& a, const BlockPart& b, int rows, int i, uint64_t at,
+                                               int head) {
+    const uint64_t row = TAIL && blockIdx.x >= a.tail ? uint64_t(b.place) * rows + i : at * a.hq + head;
+    return row * b.parts + b.split;
+}
+
 // Page of the table that list entry j stands for.
 __device__ __forceinline__ int list_page(const RowBlock& k, int j) {
     return j < k.sink_pages ? j : k.window_page + j - k.sink_pages;
@@ -112,6 +149,12 @@ __device__ __forceinline__ void zero_rows(const WindowArgs& a, const RowBlock& k
 inline uint64_t row_blocks(const WindowArgs& a, int shift) {
     if (!a.t.q_indptr) return uint64_t(a.t.batch) * ((a.r + (1u << shift) - 1) >> shift);
     return (uint64_t(a.t.rows) * a.r >> shift) + a.t.batch;
+}
+
+// Workgroups of a wide kernel.
+inline uint64_t wide_workgroups(const WindowArgs& a, int shift) {
+    const uint64_t n = row_blocks(a, shift) * a.hkv;
+    return a.tail == kNoTail ? n * a.splits : a.tail + (n - a.tail) * a.tail_parts;
 }
 
 }  // namespace

@@ -454,34 +454,54 @@ __device__ __forceinline__ void write_merged(const WindowArgs& a, uint64_t at, i
             u32x2{pack2(o[0], o[1], QT == DH_DTYPE_F16), pack2(o[2], o[3], QT == DH_DTYPE_F16)};
 }
 
-// Joins a few parts of split work (kMergeFew at most), a block of 16 rows a
-// workgroup: D / 4 lanes take a row, four elements each.  Bound by the states'
-// bytes.
+// Joins the `parts` states from `slot` on (kMergeFew at most): elements 4 col ..
+// of row `at`, head `head`.
+template <int D, uint32_t QT>
+__device__ __forceinline__ void merge_few(const WindowArgs& a, uint64_t slot, int parts, uint64_t at, int head, int col) {
+    const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
+    const f4* o = reinterpret_cast<const f4*>(a.ws_o + slot * D) + col;
+    float mx = kNegInf, sum = 0.f;
+    for (int s = 0; s < parts; ++s) mx = fmaxf(mx, ml[s][0]);
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    #pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const f2 v = ml[s];
+        const float al = v[0] == kNegInf ? 0.f : fast_exp2(v[0] - mx);
+        sum += al * v[1];
+        x += o[s * (D / 4)] * al;
+    }
+    write_merged<D, QT>(a, at, head, col, x, sum);
+}
+
+// Joins a few parts of split work, a block of 16 rows a workgroup: D / 4 lanes
+// take a row, four elements each.  Bound by the states' bytes.
 template <int D, uint32_t QT>
 __global__ __launch_bounds__(256) void window_merge_few_kernel(WindowArgs a) {
     constexpr int LPP = D / 4, G = 256 / LPP;
     const uint32_t unit = a.by_hkv(blockIdx.x);
     const RowBlock k = find_rows<4>(a, unit, int(blockIdx.x - unit * a.hkv));
-    const int grp = threadIdx.x / LPP, col = threadIdx.x % LPP;
-    const int splits = k.zero ? 0 : int(a.splits);
     #pragma unroll 1
-    for (int row = grp; row < k.nrows; row += G) {
+    for (int row = threadIdx.x / LPP; row < k.nrows; row += G) {
         int token, head;
         row_place(a, k, k.rho0 + row, token, head);
-        const uint64_t at = uint64_t(k.seq.row0) + token, slot = (at * a.hq + head) * a.splits;
-        const f2* ml = reinterpret_cast<const f2*>(a.ws_ml) + slot;
-        const f4* o = reinterpret_cast<const f4*>(a.ws_o + slot * D) + col;
-        float mx = kNegInf, sum = 0.f;
-        for (int s = 0; s < splits; ++s) mx = fmaxf(mx, ml[s][0]);
-        f4 x = {0.f, 0.f, 0.f, 0.f};
-        #pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-            const f2 v = ml[s];
-            const float al = v[0] == kNegInf ? 0.f : fast_exp2(v[0] - mx);
-            sum += al * v[1];
-            x += o[s * LPP] * al;
-        }
-        write_merged<D, QT>(a, at, head, col, x, sum);
+        const uint64_t at = uint64_t(k.seq.row0) + token;
+        merge_few<D, QT>(a, (at * a.hq + head) * a.splits, k.zero ? 0 : int(a.splits), at, head, threadIdx.x % LPP);
+    }
+}
+
+// The same for the blocks of a.tail on, 16 rows of a block a workgroup.
+template <int D, uint32_t QT, int SHIFT>
+__global__ __launch_bounds__(256) void window_merge_tail_kernel(WindowArgs a) {
+    constexpr int LPP = D / 4, G = 256 / LPP, R16 = (1 << SHIFT) / 16;
+    const uint32_t place = blockIdx.x / R16, x = a.tail + place, unit = a.by_hkv(x);
+    const RowBlock k = find_rows<SHIFT>(a, unit, int(x - unit * a.hkv));
+    const int row0 = int(blockIdx.x % R16) * 16;
+    #pragma unroll 1
+    for (int row = row0 + threadIdx.x / LPP; row < min(k.nrows, row0 + 16); row += G) {
+        int token, head;
+        row_place(a, k, k.rho0 + row, token, head);
+        merge_few<D, QT>(a, ((uint64_t(place) << SHIFT) + row) * a.tail_parts, k.zero ? 0 : int(a.tail_parts),
+                         uint64_t(k.seq.row0) + token, head, threadIdx.x % LPP);
     }
 }
 
@@ -622,6 +642,27 @@ int launch_window_merge(const WindowArgs& a, uint32_t q_dtype, uint32_t d, void*
         case 256: return launch_merge_w<256>(a, q_dtype, grid, s);
         default: return hipErrorInvalidValue;
     }
+}
+
+namespace {
+template <int D, int SHIFT>
+hipError_t launch_merge_tail_s(const WindowArgs& a, uint32_t q_dtype, uint32_t blocks, hipStream_t s) {
+    const dim3 grid(blocks << (SHIFT - 4));
+    if (q_dtype == DH_DTYPE_F16)
+        hipLaunchKernelGGL((window_merge_tail_kernel<D, DH_DTYPE_F16, SHIFT>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((window_merge_tail_kernel<D, DH_DTYPE_BF16, SHIFT>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+}  // namespace
+
+int launch_window_merge_tail(const WindowArgs& a, uint32_t q_dtype, uint32_t d, uint32_t blocks, uint32_t rows,
+                             void* stream) {
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (d == 64 && rows == 256) return launch_merge_tail_s<64, 8>(a, q_dtype, blocks, s);
+    if (d == 128 && rows == 128) return launch_merge_tail_s<128, 7>(a, q_dtype, blocks, s);
+    if (d == 256 && rows == 128) return launch_merge_tail_s<256, 7>(a, q_dtype, blocks, s);
+    return hipErrorInvalidValue;
 }
 
 }  // namespace dh

@@ -121,21 +121,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
     __shared__ __attribute__((aligned(1024))) uint8_t ring[C::RING];
     __shared__ int ids[kRingMaxPages + 2 * (P + 1)];
     const bool refused = sees_refused(a.t, blockIdx.x);
-    const uint32_t x0 = a.by_hkv(blockIdx.x);
-    const uint32_t unit = a.by_splits(x0);
-    const int split = uniform(int(x0 - unit * a.splits));
-    const RowBlock k = uniform_block(find_rows<kRingShift>(a, unit, int(blockIdx.x - x0 * a.hkv)));
+    const BlockPart b = block_part<D != 64>(a);
+    const RowBlock k = uniform_block(find_rows<kRingShift>(a, b.unit, b.head));
     report(refused, a.status);
     if (k.nrows == 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
     if (k.zero) {
-        if (a.splits == 1) zero_rows<D, DH_DTYPE_F16>(a, k);     // (else the merge writes them)
+        if (b.parts == 1) zero_rows<D, DH_DTYPE_F16>(a, k);     // (else the merge writes them)
         return;
     }
     // This workgroup's part of the page list, whole pairs.
-    int per = uniform(int(a.by_splits(uint32_t(k.pages) + a.splits - 1)));
+    int per = part_pages<D != 64>(a, b, k.pages);
     per += per & 1;
-    const int j0 = min(split * per, k.pages), n = min(min(per, k.pages - j0), int(kRingMaxPages));
+    const int j0 = min(b.split * per, k.pages), n = min(min(per, k.pages - j0), int(kRingMaxPages));
     const uint32_t npairs = uint32_t(n + 1) >> 1;
     int bad = 0;
     for (int j = tid; j < n + 2 * int(P + 1); j += 256) {
@@ -250,8 +248,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
         if ((rt * kWaves + wave) * kTileRows + c >= k.nrows) continue;
         const uint64_t at = uint64_t(k.seq.row0) + token[rt];
         const float sum = L[rt][0];
-        if (a.splits > 1) {
-            const uint64_t slot = (at * a.hq + head[rt]) * a.splits + split;
+        if (b.parts > 1) {
+            const uint64_t slot = state_slot<D != 64>(a, b, int(kRingRows), (rt * kWaves + wave) * kTileRows + c, at, head[rt]);
             #pragma unroll
             for (int e = 0; e < D / 16; ++e) *reinterpret_cast<f4*>(a.ws_o + slot * D + 16 * e + 4 * g) = O[rt][e];
             if (g == 0) *reinterpret_cast<f2*>(a.ws_ml + slot * 2) = f2{rm.m[rt], sum};
@@ -269,7 +267,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_ring_kernel(Windo
 
 template <int D>
 hipError_t launch_ring_d(const WindowArgs& a, uint32_t q_dtype, hipStream_t s) {
-    const uint64_t blocks = row_blocks(a, kRingShift) * a.splits * a.hkv;
+    const uint64_t blocks = wide_workgroups(a, kRingShift);
     if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
     const dim3 grid{uint32_t(blocks)}, block(256);
     if (q_dtype == DH_DTYPE_BF16)

@@ -334,21 +334,19 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
     __shared__ int ids[kWideMaxPages + (C::RING + C::AHEAD + 2) * NP];        // (read ahead)
     __shared__ __attribute__((aligned(16))) f2 scl[KVF == KVF_FP8 ? kWideMaxPages + 2 * NP : 1];
     const bool refused = sees_refused(a.t, blockIdx.x);
-    const uint32_t x0 = a.by_hkv(blockIdx.x);
-    const uint32_t unit = a.by_splits(x0);
-    const int split = uniform(int(x0 - unit * a.splits));
-    const RowBlock k = uniform_block(find_rows<C::SHIFT>(a, unit, int(blockIdx.x - x0 * a.hkv)));
+    const BlockPart b = block_part<true>(a);
+    const RowBlock k = uniform_block(find_rows<C::SHIFT>(a, b.unit, b.head));
     report(refused, a.status);
     if (k.nrows == 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5, c = lane & 31;
     if (k.zero) {
-        if (a.splits == 1) zero_rows<D, DH_DTYPE_F16>(a, k);     // (else the merge writes them)
+        if (b.parts == 1) zero_rows<D, DH_DTYPE_F16>(a, k);     // (else the merge writes them)
         return;
     }
     // This workgroup's part of the page list, whole tiles.
-    int per = uniform(int(a.by_splits(uint32_t(k.pages) + a.splits - 1)));
+    int per = part_pages<true>(a, b, k.pages);
     per = (per + NP - 1) / NP * NP;
-    const int j0 = min(split * per, k.pages), n = min(min(per, k.pages - j0), int(kWideMaxPages));
+    const int j0 = min(b.split * per, k.pages), n = min(min(per, k.pages - j0), int(kWideMaxPages));
     const int ntiles = (n + NP - 1) / NP;
     int bad = 0;
     for (int j = tid; j < (ntiles + C::RING + C::AHEAD + 1) * NP; j += C::THREADS) {
@@ -495,8 +493,8 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
         const float sum = pair_sum(w[rt].L) * (KVF == KVF_FP8 ? kSumUnit : 1.f);
         if (wrow + 32 * rt + c >= k.nrows) continue;
         const uint64_t at = uint64_t(k.seq.row0) + token[rt];
-        if (a.splits > 1) {
-            const uint64_t slot = (at * a.hq + head[rt]) * a.splits + split;
+        if (b.parts > 1) {
+            const uint64_t slot = state_slot<true>(a, b, int(C::ROWS), wrow + 32 * rt + c, at, head[rt]);
             #pragma unroll
             for (int e = 0; e < EB; ++e)
                 #pragma unroll
@@ -520,7 +518,7 @@ __global__ __launch_bounds__(WideCfg<D>::THREADS, WideCfg<D>::ACC ? 1 : 2) void 
 
 template <int D>
 hipError_t launch_wide_d(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, hipStream_t s) {
-    const uint64_t blocks = row_blocks(a, WideCfg<D>::SHIFT) * a.splits * a.hkv;
+    const uint64_t blocks = wide_workgroups(a, WideCfg<D>::SHIFT);
     if (blocks > 0x7FFFFFFFull) return hipErrorInvalidValue;
     const dim3 grid{uint32_t(blocks)}, block(WideCfg<D>::THREADS);
     if constexpr (D == 256) {      // (smaller heads of 16 bits: window_ring.hip)

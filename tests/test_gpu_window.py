@@ -126,6 +126,22 @@ def test_split(backend, rows, fmt, d):
     assert n > 0
 
 
+@pytest.mark.parametrize("rows,fmt,hkv,d,new", [("bf16", "bf16", 2, 128, [515]), ("f16", "fp8", 2, 128, [500, 31]),
+                                                ("bf16", "mxfp8", 2, 64, [1030]), ("f16", "f16", 2, 256, [129, 132])])
+def test_tail(backend, rows, fmt, hkv, d, new):
+    """A few blocks more than the chip holds at once: those are split by
+    themselves (64 query heads a KV head make two tokens a block, four at 64
+    dims)."""
+    kv = [2900 + n if i == 0 else 700 + n for i, n in enumerate(new)]
+    case = T.Case(29, fmt, rows, 64 * hkv, hkv, d, kv, new, row0=1, pad=2)
+    _, n = check(backend, case, 0, 0, True, max(kv))
+    assert n > 0
+    case = T.Case(30, fmt, rows, 64 * hkv, hkv, d, kv, new, row0=1, pad=2)
+    case.tables[0][90] = -1
+    case.set_tables()
+    check(backend, case, 2400, 40, False, max(kv))
+
+
 def test_long_page_lists(backend):
     """Parts of nearly as many pages as a wave's registers and a workgroup's
     list hold: batches that fill the chip, with one very long sequence."""
