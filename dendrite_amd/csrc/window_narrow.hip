@@ -412,31 +412,37 @@ __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) 
         f4 s = {0.f, 0.f, 0.f, 0.f};
         #pragma unroll
         for (int i = 0; i < KQ; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[i], qv[i], s, 0, 0, 0);
-        float x[4], mx = kNegInf;
+        float x[4];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = ok && row.sees(t0 + 4 * g + i) ? s[i] * a.scale_log2 : kNegInf;
-            mx = fmaxf(mx, x[i]);
-        }
-        mx = fmaxf(rowgroup_max(mx), m);
-        const float ref = mx == kNegInf ? 0.f : mx, alpha = fast_exp2(m - ref);
-        m = mx;
-        float ps = 0.f;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = fast_exp2(x[i] - ref);
-            ps += x[i];
-        }
-        l = l * alpha + ps;
-        #pragma unroll
-        for (int e = 0; e < EPL; ++e) O[e] *= alpha;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool keep = ok && any.sees(t0 + 4 * g + i);
+        for (int i = 0; i < 4; ++i) x[i] = s[i] * a.scale_log2;
+        if (!(ok && all_see(a, k.pmin, k.pmax, t0))) {
             #pragma unroll
-            for (int e = 0; e < EPL; ++e)
-                O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(keep ? vb[i][e] : 0.f, x[i], O[e], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                if (!(ok && row.sees(t0 + 4 * g + i))) x[i] = kNegInf;
+                const bool keep = ok && any.sees(t0 + 4 * g + i);
+                #pragma unroll
+                for (int e = 0; e < EPL; ++e) vb[i][e] = keep ? vb[i][e] : 0.f;
+            }
         }
+        // (the reference moves as in the 16-bit kernel)
+        const float lm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__ballot(lm > m + 8.f)) {
+            const float mx = rowgroup_max(lm);
+            const float mnew = mx > m + 8.f ? mx : m;
+            const float alpha = m == kNegInf ? 0.f : fast_exp2(m - mnew);
+            m = mnew;
+            l *= alpha;
+            #pragma unroll
+            for (int e = 0; e < EPL; ++e) O[e] *= alpha;
+        }
+        const float ref = m == kNegInf ? 0.f : m;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fast_exp2(x[i] - ref);
+        l += (x[0] + x[1]) + (x[2] + x[3]);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            #pragma unroll
+            for (int e = 0; e < EPL; ++e) O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[i][e], x[i], O[e], 0, 0, 0);
         if (j + 1 < pages.n) load(j + 1);
     }
     join_waves<D, DH_DTYPE_F32, NW>(a, k, split, m, rowgroup_sum(l), O, lds);
