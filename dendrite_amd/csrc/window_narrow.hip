@@ -363,7 +363,9 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
     join_waves<D, QT, NW>(a, k, split, m, rowgroup_sum(l) * (KVF == KVF_FP8 ? kSumUnit : 1.f), O, lds);
 }
 
-// f32 queries and cache: one page a step on v_mfma_f32_16x16x4_f32.
+// f32 queries and cache: one page a step on v_mfma_f32_16x16x4_f32, which bounds
+// chunks (1024 tokens x 32 heads of 128 over 2000: 488 us, 86 TFLOP/s; a large
+// library product reaches 153); few rows are bound by their pages' bytes.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) {
     constexpr int KQ = D / 4, EPL = D / 16;
@@ -396,15 +398,25 @@ __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) 
     #pragma unroll
     for (int e = 0; e < EPL; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
     float kb[KQ], vb[4][EPL];
-    auto load = [&](int j) {
+    // One wave a SIMD (256 dims) has nothing to do while K lands: it is loaded
+    // as soon as the scores are done, past the list's end too (page 0; 1024
+    // tokens x 16 heads over 2000: 474 us, and 535 at the step's end).  More waves
+    // do not gain by it (256 tokens x 32 heads of 128: 119 us, and 115).
+    constexpr bool EARLY = D == 256;
+    auto load_k = [&](int j) {
         const uint8_t* kp = a.kv + plane_offset(uint32_t(max(pages.at(j), 0)), 0, k.kv_head, a.hkv, D, 4);
-        const uint8_t* vp = kp + uint64_t(a.hkv) * (kPageSize * D * 4);
         load_dwords<KQ>(reinterpret_cast<uint32_t*>(kb), kp + (c * D + g * KQ) * 4);
+    };
+    auto load_v = [&](int j) {
+        const uint8_t* vp = a.kv + plane_offset(uint32_t(max(pages.at(j), 0)), 1, k.kv_head, a.hkv, D, 4);
         #pragma unroll
         for (int i = 0; i < 4; ++i)
             load_dwords<EPL>(reinterpret_cast<uint32_t*>(vb[i]), vp + ((4 * g + i) * D + c * EPL) * 4);
     };
-    if (pages.n > 0) load(0);
+    if (pages.n > 0) {
+        load_k(0);
+        load_v(0);
+    }
     #pragma unroll 1
     for (int j = 0; j < pages.n; ++j) {
         const bool ok = pages.at(j) >= 0;
@@ -412,6 +424,7 @@ __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) 
         f4 s = {0.f, 0.f, 0.f, 0.f};
         #pragma unroll
         for (int i = 0; i < KQ; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[i], qv[i], s, 0, 0, 0);
+        if constexpr (EARLY) load_k(j + 1);
         float x[4];
         #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = s[i] * a.scale_log2;
@@ -443,7 +456,10 @@ __global__ __launch_bounds__(64 * NW) void window_narrow32_kernel(WindowArgs a) 
         for (int i = 0; i < 4; ++i)
             #pragma unroll
             for (int e = 0; e < EPL; ++e) O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[i][e], x[i], O[e], 0, 0, 0);
-        if (j + 1 < pages.n) load(j + 1);
+        if (EARLY || j + 1 < pages.n) {
+            if constexpr (!EARLY) load_k(j + 1);
+            load_v(j + 1);
+        }
     }
     join_waves<D, DH_DTYPE_F32, NW>(a, k, split, m, rowgroup_sum(l), O, lds);
 }
