@@ -26,7 +26,7 @@
 // of 2048 and 128 first tokens in FP8 take 351 us, 0.81 PFLOP/s (16-bit caches
 // in window_ring.hip: 294).  128 rows a workgroup and two workgroups a CU beat
 // 256 rows and one (three chunks of 300 to 900 tokens over 5000: 232 us
-// against 278).
+// against 278; 202 since the last round of few blocks is split).
 #include "attend_device.hpp"
 #include "window_device.hpp"
 
