@@ -11,7 +11,7 @@
 //
 // Long calls are bound by their bytes (six prompts of 301 to 2500 tokens into
 // MXFP8, 8 heads of 128: 15 us, 4.0 TB/s; four prefixes of 2000 to 9000 read back
-// from FP8: 34 us, 4.3 TB/s), a decode step's by its dependent loads: search,
+// from FP8: 23 us, 6.3 TB/s), a decode step's by its dependent loads: search,
 // sequence, page, scale (256 tokens into FP8 pages: 7.7 us; 601 tokens read back
 // 3.4).  Rows are loaded beside the page id that says where they go.
 #include <hip/hip_runtime.h>
@@ -60,13 +60,23 @@ __device__ __forceinline__ void load8(const uint8_t* p, float (&x)[8]) {
     }
 }
 
-template <uint32_t T>
+// One store of a row that the call writes out (ROW: past the caches, which a
+// long read would only push other lines out of: four prefixes of 2000 to 9000
+// tokens from FP8 in 23 us, 6.3 TB/s, and 34 through them), or into a page, which
+// attention reads next.
+template <bool ROW, class V>
+__device__ __forceinline__ void put(V* p, V x) {
+    if constexpr (ROW) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
+template <uint32_t T, bool ROW>
 __device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8]) {
     if constexpr (T == kF32) {
         #pragma unroll
         for (int j = 0; j < 2; ++j)
-            reinterpret_cast<w4*>(p)[j] = w4{__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]),
-                                             __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])};
+            put<ROW>(reinterpret_cast<w4*>(p) + j, w4{__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]),
+                                                      __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])});
     } else {
         w4 o;
         #pragma unroll
@@ -74,7 +84,7 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8]) {
             if constexpr (T == kBF16) o[i] = __builtin_bit_cast(uint32_t, b2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
             else o[i] = __builtin_bit_cast(uint32_t, h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
         }
-        *reinterpret_cast<w4*>(p) = o;
+        put<ROW>(reinterpret_cast<w4*>(p), o);
     }
 }
 
@@ -257,7 +267,7 @@ __global__ __launch_bounds__(256) void append_tokens_kernel(TokenCopyArgs a) {
         #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int t = i * RPI + lr;
-            if (t >= k.lo && t < k.hi) store8<FMT>(dst + t * (D * DB), x[i]);
+            if (t >= k.lo && t < k.hi) store8<FMT, false>(dst + t * (D * DB), x[i]);
         }
     }
 }
@@ -306,7 +316,7 @@ __global__ __launch_bounds__(256) void read_tokens_kernel(TokenCopyArgs a) {
     #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const int t = i * RPI + lr;
-        if (t >= k.lo && t < k.hi) store8<DST>(dst + uint64_t(k.row0 + t) * stride, x[i]);
+        if (t >= k.lo && t < k.hi) store8<DST, true>(dst + uint64_t(k.row0 + t) * stride, x[i]);
     }
 }
 
