@@ -1347,6 +1347,7 @@ struct WindowPlan {
     uint32_t splits;
     uint32_t window, sinks;
     uint32_t rows;             // of a block
+    bool once;                 // WindowArgs::once
     uint32_t tail, tail_blocks, tail_parts;     // wide blocks split by themselves (WindowArgs)
     size_t o_bytes, bytes;     // workspace: O, all
 };
@@ -1437,6 +1438,12 @@ WindowPlan plan_window(const dh_attn_config& c, const dh_token_tables& t, uint32
     // 64 heads of 128 over 2048: 90 us, and 111 whole (bf16), 106 and 133 (FP8);
     // 2200 x 16 heads of 256: 140 and 200.
     w.rows = uint32_t(block);
+    // Pages that one block reads, more of them than the last level of cache (256
+    // MiB) holds: V is better not kept (64 sequences, window 4096, bf16, 32 heads
+    // of 128: 152 us, and 167 kept).  What several blocks read is (32 sequences of 6
+    // tokens, window 2001, 32 heads of 128: 51 us, and 60 not kept).
+    const uint64_t page_bytes = 2ull * c.num_kv_heads * 16 * c.head_dim * (codes ? 1 : c.q_dtype == DH_DTYPE_F32 ? 4 : 2);
+    w.once = !t.q_indptr && r <= 16 && t.batch_size * pages * page_bytes > (256ull << 20);
     w.tail = dh::kNoTail;
     const uint64_t slots = wide_slots(c.head_dim, w.ring), rounds = filled / slots;
     if (w.wide && w.splits == 1 && !(w.ring && c.head_dim == 64) && rounds >= 1 && rounds <= 4 && filled > rounds * slots) {
@@ -1526,6 +1533,7 @@ dh_status dh_attend_window(dh_backend* be, const dh_pool* pool, const dh_attn_co
     a.by_hkv = dh::Divisor::of(a.hkv);
     a.by_r = dh::Divisor::of(r);
     a.by_splits = dh::Divisor::of(w.splits);
+    a.once = w.once ? 1u : 0u;
     a.tail = w.tail;
     a.tail_parts = w.tail_parts;
     a.by_tail = dh::Divisor::of(std::max(1u, w.tail_parts));

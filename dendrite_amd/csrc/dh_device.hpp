@@ -270,6 +270,7 @@ struct WindowArgs {
     // Wide blocks tail, tail + 1, ... (KV heads fastest) are split tail_parts
     // ways, the others not (splits 1); kNoTail: none.  Row i of the block, part
     // s: state ((block - tail) rows + i) tail_parts + s of ws_o / ws_ml.
+    uint32_t once;               // narrow: V is read by one block, and not in the caches
     uint32_t tail, tail_parts;
     Divisor by_tail;
     int32_t* status;

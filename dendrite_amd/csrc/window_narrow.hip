@@ -13,8 +13,8 @@
 // writes (O, m, L) in f32 and a merge kernel joins them.
 //
 // Every page is read once per block.  Large batches are bound by those bytes (64
-// sequences under a window of 4096, bf16, 32 heads of 128: 166 us, 5.6 TB/s; 256
-// in FP8 under 1024 + 64, 64 heads: 109 us, 4.7; one token over 100 000, f16, 16
+// sequences under a window of 4096, bf16, 32 heads of 128: 152 us, 6.1 TB/s; 256
+// in FP8 under 1024 + 64, 64 heads: 101 us, 5.1; one token over 100 000, f16, 16
 // heads of 256: 38 us, 5.3), blocks of several tokens by 8-bit conversion (32
 // sequences of 3 to 9 tokens in MXFP8, 16 heads of 256: 42 us), small calls by
 // their dependent loads (one f32 token under a window of 256: 9.1 us).
@@ -23,6 +23,34 @@
 
 namespace dh {
 namespace {
+
+// Whether the lanes' shares of a page's V make whole lines of its rows (8 or 16
+// bytes each): only then can V be loaded without leaving lines behind, since
+// parts of lines would be fetched again.
+template <int D, uint32_t KVF>
+constexpr bool kWholeLines = D / 16 * (PageRaw<D, KVF>::FP8 ? 1 : 2) == 8 || D / 16 * (PageRaw<D, KVF>::FP8 ? 1 : 2) == 16;
+
+// A page's V as load_page_v has it, in loads that leave no line behind.
+template <int D, uint32_t KVF>
+__device__ __forceinline__ void load_v_once(PageRaw<D, KVF>& r, const AttendArgs& kv, uint32_t page, uint32_t head, int g,
+                                            int c) {
+    using R = PageRaw<D, KVF>;
+    constexpr int EB = R::FP8 ? 1 : 2, W = R::EPL * EB / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(W)));
+    const uint8_t* p = kv.kv + plane_offset(page, 1, head, kv.hkv, D, EB) + (4 * g * D + c * R::EPL) * EB;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const words v = __builtin_nontemporal_load(reinterpret_cast<const words*>(p + j * D * EB));
+        #pragma unroll
+        for (int w = 0; w < W; ++w) r.v[j][w] = v[w];
+    }
+    if constexpr (KVF == KVF_MX) {
+        const uint8_t* s = reinterpret_cast<const uint8_t*>(kv.scales) +
+                           ((uint64_t(page) * 2 + 1) * kv.hkv + head) * uint64_t(kPageSize) * R::G;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) r.vsc[j] = s[(4 * g + j) * R::G + c * R::EPL / 32];
+    }
+}
 
 // The page ids of a wave's part of the list, kNarrowWavePages at most, in
 // registers (lane l holds entries l, l + 64, ...): -1 for an entry outside the
@@ -157,7 +185,7 @@ __device__ __forceinline__ RowBlock workgroup_rows(const WindowArgs& a, int& spl
 template <int D, bool CODES>
 constexpr int kNarrowPerSimd = !CODES ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4;
 
-template <int D, uint32_t KVF, bool F16, int NW>
+template <int D, uint32_t KVF, bool F16, int NW, bool ONCE>
 __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>)) void window_narrow_kernel(WindowArgs a) {
     using R = PageRaw<D, KVF>;
     constexpr int KB = D / 32, EPL = D / 16;
@@ -216,19 +244,20 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
             if constexpr (KVF == KVF_FP8) ks[q] = id < 0 ? 1.f : bsc[(uint64_t(pg) * 2 + 0) * a.hkv + k.kv_head];
         }
     };
-    auto load_v = [&](int pair) {
+    auto load_values = [&](int pair) {
         #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int id = pages.at(2 * pair + q);
             const uint32_t pg = uint32_t(max(id, 0));
-            load_page_v<D, KVF>(pr[q], kv, pg, k.kv_head, g, c);
+            if constexpr (ONCE) load_v_once<D, KVF>(pr[q], kv, pg, k.kv_head, g, c);
+            else load_page_v<D, KVF>(pr[q], kv, pg, k.kv_head, g, c);
             if constexpr (KVF == KVF_FP8) vs[q] = id < 0 ? 1.f : bsc[(uint64_t(pg) * 2 + 1) * a.hkv + k.kv_head];
         }
     };
     const int npairs = (pages.n + 1) >> 1;
     if (npairs > 0) {
         load_k(0);
-        load_v(0);
+        load_values(0);
     }
     #pragma unroll 1
     for (int pi = 0; pi < npairs; ++pi) {
@@ -358,7 +387,7 @@ __global__ __launch_bounds__(64 * NW, (kNarrowPerSimd<D, PageRaw<D, KVF>::FP8>))
             for (int e = 0; e < EPL; ++e)
                 product(e, [&](int q, int j) __attribute__((always_inline)) { return pr[q].v[j][e >> 1]; });
         }
-        if (refill) load_v(pi + 1);
+        if (refill) load_values(pi + 1);
     }
     join_waves<D, QT, NW>(a, k, split, m, rowgroup_sum(l) * (KVF == KVF_FP8 ? kSumUnit : 1.f), O, lds);
 }
@@ -582,30 +611,34 @@ __global__ __launch_bounds__(NT) void window_merge_kernel(WindowArgs a) {
     write_merged<D, QT>(a, at, head, col, x, sum);
 }
 
+template <int D, uint32_t KVF, bool F16, int NW>
+hipError_t launch_narrow_f(const WindowArgs& a, dim3 grid, hipStream_t s) {
+    if constexpr (kWholeLines<D, KVF>) {
+        if (a.once) {
+            hipLaunchKernelGGL((window_narrow_kernel<D, KVF, F16, NW, true>), grid, dim3(64 * NW), 0, s, a);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((window_narrow_kernel<D, KVF, F16, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    return hipGetLastError();
+}
+
 template <int D, int NW>
 hipError_t launch_narrow_w(const WindowArgs& a, uint32_t q_dtype, uint32_t fmt, dim3 grid, hipStream_t s) {
-    const dim3 block(64 * NW);
-    if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_FP8)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, false, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_FP8)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_FP8, true, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_MX)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, false, NW>), grid, block, 0, s, a);
-    else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_MX)
-        hipLaunchKernelGGL((window_narrow_kernel<D, KVF_MX, true, NW>), grid, block, 0, s, a);
-    else if constexpr (NW <= int(narrow_waves(D, false))) {
-        if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32)
-            hipLaunchKernelGGL((window_narrow32_kernel<D, NW>), grid, block, 0, s, a);
-        else if (q_dtype == DH_DTYPE_BF16 && fmt == KVF_BF16)
-            hipLaunchKernelGGL((window_narrow_kernel<D, KVF_BF16, false, NW>), grid, block, 0, s, a);
-        else if (q_dtype == DH_DTYPE_F16 && fmt == KVF_F16)
-            hipLaunchKernelGGL((window_narrow_kernel<D, KVF_F16, true, NW>), grid, block, 0, s, a);
-        else
-            return hipErrorInvalidValue;
-    } else {
-        return hipErrorInvalidValue;
+    const bool bf16 = q_dtype == DH_DTYPE_BF16, f16 = q_dtype == DH_DTYPE_F16;
+    if (bf16 && fmt == KVF_FP8) return launch_narrow_f<D, KVF_FP8, false, NW>(a, grid, s);
+    if (f16 && fmt == KVF_FP8) return launch_narrow_f<D, KVF_FP8, true, NW>(a, grid, s);
+    if (bf16 && fmt == KVF_MX) return launch_narrow_f<D, KVF_MX, false, NW>(a, grid, s);
+    if (f16 && fmt == KVF_MX) return launch_narrow_f<D, KVF_MX, true, NW>(a, grid, s);
+    if constexpr (NW <= int(narrow_waves(D, false))) {
+        if (bf16 && fmt == KVF_BF16) return launch_narrow_f<D, KVF_BF16, false, NW>(a, grid, s);
+        if (f16 && fmt == KVF_F16) return launch_narrow_f<D, KVF_F16, true, NW>(a, grid, s);
+        if (q_dtype == DH_DTYPE_F32 && fmt == KVF_F32) {
+            hipLaunchKernelGGL((window_narrow32_kernel<D, NW>), grid, dim3(64 * NW), 0, s, a);
+            return hipGetLastError();
+        }
     }
-    return hipGetLastError();
+    return hipErrorInvalidValue;
 }
 
 template <int D>
