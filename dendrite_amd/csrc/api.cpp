@@ -1358,7 +1358,8 @@ uint32_t wide_slots(uint32_t head_dim, bool ring) { return head_dim == 256 ? 256
 // Parts of a wide block's page list: the fewest microseconds by a model of the
 // wide kernels, fitted to their times.  A full chip takes head_dim / 256 us a
 // page of every block, three quarters of that half full, and 14 pages' time to
-// start; a last round that does not fill it counts half empty; the parts' states are written and read at 4.5 TB/s, 4 us the launch.
+// start; a last round that does not fill it counts half empty; the parts' states
+// are written and read at 4.5 TB/s, 4 us the launch.
 // (Tokens x heads of 128 over a 16-bit context, in one part and as chosen: 256 x
 // 64 over a window of 2048 55 and 46 us; 400 x 32 over 12000 134 and 97; 1100 x
 // 32 284 and 243.)
